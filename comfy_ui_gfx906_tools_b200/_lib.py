@@ -72,6 +72,16 @@ SIGNATURES = {
     "attention_max_tiles": (_c_int, []),
     "w4a4_gemm_exact_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int]),
     "w4a4_gemm_exact_splits": (_c_int, [_c_int, _c_int, _c_int, _c_int]),
+    "adamw_step": (_c_int, [_c_void_p] * 7 + [_c_int] * 4 + [_c_int64] + [ctypes.c_double] * 5 +
+                   [_c_void_p, _c_void_p]),
+    "adamw_moment_values": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_void_p]),
+    "qk_norm_rope": (_c_int, [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] +
+                     [_c_void_p] * 4 + [_c_int] * 5 + [_c_void_p, _c_int, ctypes.c_double, _c_int, ctypes.c_float,
+                                                       _c_void_p]),
+    "qk_norm_rope_backward": (_c_int, [_c_void_p] * 8 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] +
+                              [_c_void_p] * 6 + [_c_int] * 5 + [_c_void_p, _c_int, ctypes.c_double, _c_int,
+                                                                ctypes.c_float, _c_void_p, _c_size_t, _c_void_p]),
+    "qk_norm_rope_workspace_bytes": (_c_size_t, [_c_int]),
     "w4a4_gemm_exact": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                                  _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_size_t, _c_void_p]),
 }

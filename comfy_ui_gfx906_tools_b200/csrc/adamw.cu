@@ -1,0 +1,314 @@
+// One AdamW step over many tensors in one launch, first and second moments in
+// float32 or in 8 bits with one float32 scale per 256 elements.
+//
+//   m <- b1 m + (1 - b1) g          v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit moments are companded: a code c stands for the value c |c| s, so the
+// steps between neighbouring codes shrink towards zero. The first moment holds
+// c in [-127, 127]; the second moment holds its square root, c in [0, 255],
+// and a positive one keeps at least the code 1: rounded to 0 it would leave
+// the next update of that element nothing but eps to divide by. s is the
+// block's largest magnitude over 127^2 (255^2). Every step of the coding is a
+// correctly rounded float32 operation, so its result is the same wherever it
+// is computed.
+//
+// Memory-bound: p is read and written, g read, each moment read and written.
+// A warp owns 256 consecutive elements, which is one block of the 8-bit form:
+// its largest magnitude is one warp-wide integer maximum (magnitudes order as
+// their bit patterns do, and a NaN lies above every number, so it is not lost).
+// A lane holds elements 4 l .. 4 l + 3 of each 128-element half, so every
+// access of the warp is one contiguous run.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace gfx {
+namespace adamw {
+
+constexpr int kWarps = 8;
+constexpr int kBlock = 256;  // elements per warp step = elements per 8-bit scale
+
+struct Args {
+  AdamwTensor t[kAdamwMaxTensors];
+  int count;
+  int blocks_per_cta;  // 256-element blocks one CTA takes
+  const float* grad_scale;
+  float beta1, one_minus_beta1, beta2, one_minus_beta2, decay, step_size, root_scale, eps;
+};
+
+template <typename T>
+struct Quad;
+template <>
+struct Quad<float> {
+  using V = float4;
+  static __device__ __forceinline__ void unpack(const V& v, float (&f)[4]) {
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  }
+  static __device__ __forceinline__ V pack(const float (&f)[4]) { return make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <typename T, typename T2>
+struct Quad16 {
+  using V = uint2;
+  static __device__ __forceinline__ void unpack(const V& v, float (&f)[4]) {
+    const T2 a = *reinterpret_cast<const T2*>(&v.x), b = *reinterpret_cast<const T2*>(&v.y);
+    f[0] = to_f32<T>(a.x), f[1] = to_f32<T>(a.y), f[2] = to_f32<T>(b.x), f[3] = to_f32<T>(b.y);
+  }
+  static __device__ __forceinline__ V pack(const float (&f)[4]) {
+    T2 a, b;
+    a.x = from_f32<T>(f[0]), a.y = from_f32<T>(f[1]), b.x = from_f32<T>(f[2]), b.y = from_f32<T>(f[3]);
+    return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+};
+template <>
+struct Quad<__half> : Quad16<__half, __half2> {};
+template <>
+struct Quad<__nv_bfloat16> : Quad16<__nv_bfloat16, __nv_bfloat162> {};
+
+// Elements e .. e + 3 of a tensor of n; vec: the tensor's arrays are 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load4(const void* base, long long e, long long n, bool vec, float (&f)[4]) {
+  const T* p = static_cast<const T*>(base) + e;
+  if (vec && e + 4 <= n) {
+    Quad<T>::unpack(*reinterpret_cast<const typename Quad<T>::V*>(p), f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = e + j < n ? to_f32<T>(p[j]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(void* base, long long e, long long n, bool vec, const float (&f)[4]) {
+  T* p = static_cast<T*>(base) + e;
+  if (vec && e + 4 <= n) {
+    *reinterpret_cast<typename Quad<T>::V*>(p) = Quad<T>::pack(f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e + j < n) p[j] = from_f32<T>(f[j]);
+  }
+}
+
+__device__ __forceinline__ uint32_t load_codes(const void* base, long long e, long long n, bool vec) {
+  const uint8_t* p = static_cast<const uint8_t*>(base) + e;
+  if (vec && e + 4 <= n) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (e + j < n) w |= (uint32_t)p[j] << (8 * j);
+  return w;
+}
+
+__device__ __forceinline__ void store_codes(void* base, long long e, long long n, bool vec, uint32_t w) {
+  uint8_t* p = static_cast<uint8_t*>(base) + e;
+  if (vec && e + 4 <= n) {
+    *reinterpret_cast<uint32_t*>(p) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e + j < n) p[j] = (uint8_t)(w >> (8 * j));
+  }
+}
+
+// The value that code c stands for under scale s: first moment, or root of the second.
+__device__ __forceinline__ float first_value(uint32_t w, int j, float s) {
+  const int c = (int)(int8_t)(w >> (8 * j));
+  return __fmul_rn((float)(c * abs(c)), s);
+}
+__device__ __forceinline__ float root_value(uint32_t w, int j, float s) {
+  const int c = (int)((w >> (8 * j)) & 0xFFu);
+  return __fmul_rn((float)(c * c), s);
+}
+
+// Scale of a block whose largest magnitude has these bits, and its reciprocal. A largest magnitude too small
+// for a normal scale codes the block as zeros; an infinite or NaN one gives a NaN scale, which decodes as NaN.
+__device__ __forceinline__ float block_scale(uint32_t amax_bits, float over, float& inv) {
+  const float s = __fmul_rn(__uint_as_float(amax_bits), over);
+  inv = 0.0f;
+  if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  if (s < 1.17549435e-38f) return 0.0f;
+  inv = __fdiv_rn(1.0f, s);
+  return s;
+}
+
+__device__ __forceinline__ uint32_t code_of(float magnitude, float inv, int top) {
+  return (uint32_t)min(__float2int_rn(__fsqrt_rn(__fmul_rn(magnitude, inv))), top);
+}
+
+template <typename P, typename G, bool k8>
+__global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ Args a) {
+  // the tensor of this CTA: the last whose first CTA is not past it
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.t[mid].first_cta <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  const AdamwTensor& t = a.t[lo];
+  const long long n = t.n, blocks = (n + kBlock - 1) / kBlock;
+  const long long b0 = (long long)((int)blockIdx.x - t.first_cta) * a.blocks_per_cta;
+  const long long b1 = b0 + a.blocks_per_cta < blocks ? b0 + a.blocks_per_cta : blocks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool vec = t.aligned != 0;
+  const float gs = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
+
+  for (long long b = b0 + warp; b < b1; b += kWarps) {
+    float m[2][4], v[2][4], p[2][4];
+    const float ms = k8 ? t.m_scale[b] : 0.0f, vs = k8 ? t.v_scale[b] : 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long e = b * kBlock + h * 128 + lane * 4;
+      float g[4];
+      load4<P>(t.p, e, n, vec, p[h]);
+      load4<G>(t.g, e, n, vec, g);
+      if constexpr (k8) {
+        const uint32_t mw = load_codes(t.m, e, n, vec), vw = load_codes(t.v, e, n, vec);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[h][j] = first_value(mw, j, ms);
+          const float r = root_value(vw, j, vs);
+          v[h][j] = __fmul_rn(r, r);
+        }
+      } else {
+        load4<float>(t.m, e, n, vec, m[h]);
+        load4<float>(t.v, e, n, vec, v[h]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float gj = __fmul_rn(g[j], gs);
+        m[h][j] = __fadd_rn(__fmul_rn(m[h][j], a.beta1), __fmul_rn(gj, a.one_minus_beta1));
+        v[h][j] = __fadd_rn(__fmul_rn(v[h][j], a.beta2), __fmul_rn(__fmul_rn(gj, gj), a.one_minus_beta2));
+      }
+      if constexpr (!k8) {
+        store4<float>(t.m, e, n, vec, m[h]);
+        store4<float>(t.v, e, n, vec, v[h]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[h][j] = __fsqrt_rn(v[h][j]);
+        p[h][j] = p[h][j] * a.decay - a.step_size * (m[h][j] / (v[h][j] * a.root_scale + a.eps));
+      }
+      store4<P>(t.p, e, n, vec, p[h]);
+    }
+    if constexpr (k8) {
+      uint32_t mb = 0, vb = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mb = max(mb, __float_as_uint(m[h][j]) & 0x7FFFFFFFu);
+          vb = max(vb, __float_as_uint(v[h][j]) & 0x7FFFFFFFu);
+        }
+      mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+      vb = __reduce_max_sync(0xFFFFFFFFu, vb);
+      float mi, vi;
+      const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi), vs1 = block_scale(vb, 1.0f / 65025.0f, vi);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long e = b * kBlock + h * 128 + lane * 4;
+        uint32_t mw = 0, vw = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = (int)code_of(fabsf(m[h][j]), mi, 127);
+          mw |= ((uint32_t)(m[h][j] < 0.0f ? -c : c) & 0xFFu) << (8 * j);
+          uint32_t d = code_of(v[h][j], vi, 255);
+          if (vi > 0.0f && v[h][j] > 0.0f && d == 0) d = 1;
+          vw |= d << (8 * j);
+        }
+        store_codes(t.m, e, n, vec, mw);
+        store_codes(t.v, e, n, vec, vw);
+      }
+      if (lane == 0) {
+        t.m_scale[b] = ms1;
+        t.v_scale[b] = vs1;
+      }
+    }
+  }
+}
+
+// The values that 8-bit moments stand for (second: codes are roots, the value is squared).
+template <bool kSecond>
+__global__ void __launch_bounds__(kWarps * 32) moment_values_kernel(const void* codes, const float* scale, float* out,
+                                                                    long long n, int vec) {
+  const int lane = threadIdx.x & 31;
+  const long long blocks = (n + kBlock - 1) / kBlock;
+  for (long long b = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); b < blocks; b += (long long)gridDim.x * kWarps) {
+    const float s = scale[b];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long e = b * kBlock + h * 128 + lane * 4;
+      const uint32_t w = load_codes(codes, e, n, vec != 0);
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = kSecond ? root_value(w, j, s) : first_value(w, j, s);
+        if (kSecond) f[j] = __fmul_rn(f[j], f[j]);
+      }
+      store4<float>(out, e, n, vec != 0, f);
+    }
+  }
+}
+
+}  // namespace adamw
+
+template <typename P, typename G>
+static int launch_adamw_t(const adamw::Args& a, bool bits8, int ctas, cudaStream_t st) {
+  if (bits8)
+    adamw::adamw_kernel<P, G, true><<<ctas, adamw::kWarps * 32, 0, st>>>(a);
+  else
+    adamw::adamw_kernel<P, G, false><<<ctas, adamw::kWarps * 32, 0, st>>>(a);
+  return check_launch("adamw_kernel");
+}
+
+template <typename P>
+static int launch_adamw_g(int g_dtype, const adamw::Args& a, bool bits8, int ctas, cudaStream_t st) {
+  if (g_dtype == GFX_DTYPE_F32) return launch_adamw_t<P, float>(a, bits8, ctas, st);
+  if (g_dtype == GFX_DTYPE_F16) return launch_adamw_t<P, __half>(a, bits8, ctas, st);
+  return launch_adamw_t<P, __nv_bfloat16>(a, bits8, ctas, st);
+}
+
+int launch_adamw(const AdamwTensor* tensors, int count, int p_dtype, int g_dtype, bool bits8, const AdamwScalars& c,
+                 cudaStream_t st, int sms) {
+  adamw::Args a;
+  a.grad_scale = c.grad_scale;
+  a.beta1 = c.beta1, a.one_minus_beta1 = c.one_minus_beta1, a.beta2 = c.beta2, a.one_minus_beta2 = c.one_minus_beta2;
+  a.decay = c.decay, a.step_size = c.step_size, a.root_scale = c.root_scale, a.eps = c.eps;
+  (void)sms;
+  a.blocks_per_cta = adamw::kWarps;
+  for (int i = 0; i < count;) {
+    // as many tensors as one launch's arguments hold; empty ones take no CTA
+    a.count = 0;
+    long long ctas = 0;
+    for (; i < count && a.count < kAdamwMaxTensors; ++i) {
+      const long long blocks = (tensors[i].n + adamw::kBlock - 1) / adamw::kBlock;
+      if (blocks == 0) continue;
+      const long long need = (blocks + a.blocks_per_cta - 1) / a.blocks_per_cta;
+      if (ctas + need > 0x7FFFFFFFll) break;  // the grid's limit: the rest goes into the next launch
+      a.t[a.count] = tensors[i];
+      a.t[a.count].first_cta = (int)ctas;
+      ++a.count;
+      ctas += need;
+    }
+    if (a.count == 0) continue;
+    int rc;
+    if (p_dtype == GFX_DTYPE_F32)
+      rc = launch_adamw_g<float>(g_dtype, a, bits8, (int)ctas, st);
+    else if (p_dtype == GFX_DTYPE_F16)
+      rc = launch_adamw_g<__half>(g_dtype, a, bits8, (int)ctas, st);
+    else
+      rc = launch_adamw_g<__nv_bfloat16>(g_dtype, a, bits8, (int)ctas, st);
+    if (rc) return rc;
+  }
+  return GFX_OK;
+}
+
+int launch_moment_values(const void* codes, const float* scale, float* out, long long n, int second, int vec,
+                         cudaStream_t st, int sms) {
+  const long long need = ((n + adamw::kBlock - 1) / adamw::kBlock + adamw::kWarps - 1) / adamw::kWarps;
+  const int ctas = (int)(need < (long long)sms * 8 ? need : (long long)sms * 8);
+  if (second)
+    adamw::moment_values_kernel<true><<<ctas, adamw::kWarps * 32, 0, st>>>(codes, scale, out, n, vec);
+  else
+    adamw::moment_values_kernel<false><<<ctas, adamw::kWarps * 32, 0, st>>>(codes, scale, out, n, vec);
+  return check_launch("moment_values_kernel");
+}
+
+}  // namespace gfx

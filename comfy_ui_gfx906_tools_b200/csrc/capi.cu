@@ -1,10 +1,13 @@
 // C ABI of the library (declared in include/gfx906_b200.h): argument checks
 // mirroring the reference binding (nodes/ComfyUI-Gfx906Int4/csrc/binding.cpp),
 // per-device caches, TMA descriptor encoding, dispatch to the kernels.
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
+#include <vector>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -612,6 +615,200 @@ int hadamard_rotate(const void* x, int x_dtype, const float* sign, void* out, in
   if (rows == 0) return GFX_OK;
   if (!x || !sign || !out) return set_error(GFX_ERR_INVALID, "hadamard_rotate: null pointer");
   return gfx::launch_hadamard_rotate(x, x_dtype, sign, out, out_dtype, rows, K, group, (cudaStream_t)stream);
+}
+
+int adamw_step(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
+               float* const* v_scale, const int64_t* numel, int count, int p_dtype, int g_dtype, int state_bits,
+               int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+               const float* grad_scale, gfx_stream_t stream) {
+  const char* fn = "adamw_step";
+  if (count < 0) return set_error(GFX_ERR_INVALID, "%s: count must be >= 0, got %d", fn, count);
+  if (!valid_dtype(p_dtype) || !valid_dtype(g_dtype))
+    return set_error(GFX_ERR_INVALID, "%s: dtype codes must be 0 (f32) / 1 (f16) / 2 (bf16), got p %d g %d", fn, p_dtype,
+                     g_dtype);
+  if (state_bits != 32 && state_bits != 8)
+    return set_error(GFX_ERR_INVALID, "%s: state_bits must be 32 or 8, got %d", fn, state_bits);
+  if (step < 1) return set_error(GFX_ERR_INVALID, "%s: step counts from 1, got %lld", fn, (long long)step);
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
+    return set_error(GFX_ERR_INVALID, "%s: betas must be in [0, 1), got %g, %g", fn, beta1, beta2);
+  if (!(lr >= 0.0) || !(eps >= 0.0) || !(weight_decay >= 0.0))
+    return set_error(GFX_ERR_INVALID, "%s: lr, eps and weight_decay must be >= 0, got %g, %g, %g", fn, lr, eps,
+                     weight_decay);
+  if (count == 0) return GFX_OK;
+  const bool b8 = state_bits == 8;
+  if (!p || !g || !m || !v || !numel || (b8 && (!m_scale || !v_scale)))
+    return set_error(GFX_ERR_INVALID, "%s: null pointer array", fn);
+  static const int kSize[3] = {4, 2, 2};
+  try {
+    std::vector<AdamwTensor> t((size_t)count);
+    for (int i = 0; i < count; ++i) {
+      AdamwTensor& x = t[(size_t)i];
+      x = AdamwTensor{p[i], g[i], m[i], v[i], b8 ? m_scale[i] : nullptr, b8 ? v_scale[i] : nullptr, numel[i], 0, 0};
+      if (x.n < 0) return set_error(GFX_ERR_INVALID, "%s: tensor %d has %lld elements", fn, i, (long long)x.n);
+      if (x.n == 0) continue;
+      if (!x.p || !x.g || !x.m || !x.v || (b8 && (!x.m_scale || !x.v_scale)))
+        return set_error(GFX_ERR_INVALID, "%s: null pointer in tensor %d", fn, i);
+      const uintptr_t pa = reinterpret_cast<uintptr_t>(x.p), ga = reinterpret_cast<uintptr_t>(x.g);
+      const uintptr_t ma = reinterpret_cast<uintptr_t>(x.m), va = reinterpret_cast<uintptr_t>(x.v);
+      const uintptr_t sa = reinterpret_cast<uintptr_t>(x.m_scale) | reinterpret_cast<uintptr_t>(x.v_scale);
+      if (pa % kSize[p_dtype] || ga % kSize[g_dtype] || (!b8 && ((ma | va) & 3)) || (sa & 3))
+        return set_error(GFX_ERR_INVALID, "%s: an array of tensor %d is not aligned to its element size", fn, i);
+      x.aligned = ((pa | ga | ma | va) & 15) == 0;
+    }
+    AdamwScalars c;
+    c.grad_scale = grad_scale;
+    c.beta1 = (float)beta1, c.one_minus_beta1 = (float)(1.0 - beta1);
+    c.beta2 = (float)beta2, c.one_minus_beta2 = (float)(1.0 - beta2);
+    c.decay = (float)(1.0 - lr * weight_decay);
+    c.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    c.root_scale = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    c.eps = (float)eps;
+    return launch_adamw(t.data(), count, p_dtype, g_dtype, b8, c, reinterpret_cast<cudaStream_t>(stream),
+                        sm_count(current_device()));
+  } catch (const std::bad_alloc&) {
+    return set_error(GFX_ERR_INVALID, "%s: out of host memory for %d tensors", fn, count);
+  }
+}
+
+int adamw_moment_values(const void* codes, const float* scale, float* out, int64_t n, int second, gfx_stream_t stream) {
+  const char* fn = "adamw_moment_values";
+  if (n < 0) return set_error(GFX_ERR_INVALID, "%s: n must be >= 0, got %lld", fn, (long long)n);
+  if (n == 0) return GFX_OK;
+  if (!codes || !scale || !out) return set_error(GFX_ERR_INVALID, "%s: null pointer", fn);
+  if (((uintptr_t)scale & 3) || ((uintptr_t)out & 3))
+    return set_error(GFX_ERR_INVALID, "%s: scale and out must be 4-byte aligned", fn);
+  const int vec = (((uintptr_t)codes & 3) | ((uintptr_t)out & 15)) == 0;
+  return launch_moment_values(codes, scale, out, n, second, vec, (cudaStream_t)stream, sm_count(current_device()));
+}
+
+// The arguments that both directions share, checked and laid down in `a`.
+static int rope_common(const char* fn, RopeArgs* a, int dtype, const void* positions, int pos_dtype,
+                       const int64_t* pos_strides, const void* q_scale, const void* k_scale, int scale_dtype, int B,
+                       int Hq, int Hk, int L, int D, const int* axes_dims, int n_axes, double theta, int interleaved,
+                       float eps) {
+  if (!valid_dtype(dtype) || !valid_dtype(scale_dtype))
+    return set_error(GFX_ERR_INVALID, "%s: dtype codes must be 0 (f32) / 1 (f16) / 2 (bf16), got %d and scale %d", fn,
+                     dtype, scale_dtype);
+  if (pos_dtype < 0 || pos_dtype > 2)
+    return set_error(GFX_ERR_INVALID, "%s: positions are float32 (0), int32 (1) or int64 (2), got %d", fn, pos_dtype);
+  if (B < 0 || Hq < 0 || Hk < 0 || L < 0)
+    return set_error(GFX_ERR_INVALID, "%s: expected B, Hq, Hk, L >= 0; got B=%d Hq=%d Hk=%d L=%d", fn, B, Hq, Hk, L);
+  if (D <= 0 || D % 8 != 0 || D > kRopeMaxDim)
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: D must be a multiple of 8 up to %d, got %d", fn, kRopeMaxDim, D);
+  if (!axes_dims || n_axes < 1 || n_axes > kRopeMaxAxes)
+    return set_error(GFX_ERR_INVALID, "%s: between 1 and %d axes, got %d", fn, kRopeMaxAxes, n_axes);
+  long long sum = 0;
+  for (int i = 0; i < n_axes; ++i) {
+    if (axes_dims[i] < 2 || axes_dims[i] % 2 != 0)
+      return set_error(GFX_ERR_INVALID, "%s: axes_dims must be even and at least 2, got %d", fn, axes_dims[i]);
+    sum += axes_dims[i];
+  }
+  if (sum > D) return set_error(GFX_ERR_INVALID, "%s: axes_dims add up to %lld, more than D=%d", fn, sum, D);
+  if (!interleaved && sum % 8 != 0)
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: split halves need sum(axes_dims) %% 8 == 0, got %lld", fn, sum);
+  if (!(theta > 0.0) || !(eps >= 0.0f))
+    return set_error(GFX_ERR_INVALID, "%s: theta must be > 0 and eps >= 0, got %g, %g", fn, theta, (double)eps);
+  if (!pos_strides) return set_error(GFX_ERR_INVALID, "%s: null pointer among the positions' strides", fn);
+  if ((long long)B * L > 0 && Hq + Hk > 0) {
+    if (!positions) return set_error(GFX_ERR_INVALID, "%s: positions is a null pointer", fn);
+    if ((uintptr_t)positions & (pos_dtype == kPositionI64 ? 7 : 3))
+      return set_error(GFX_ERR_INVALID, "%s: positions are not aligned to their element size", fn);
+  }
+  const uintptr_t es = scale_dtype == GFX_DTYPE_F32 ? 3 : 1;
+  if (((uintptr_t)q_scale & es) || ((uintptr_t)k_scale & es))
+    return set_error(GFX_ERR_INVALID, "%s: a scale is not aligned to its element size", fn);
+  memset(a, 0, sizeof(*a));
+  rope_frequencies(a, axes_dims, n_axes, theta);
+  a->heads[0] = Hq, a->heads[1] = Hk;
+  a->B = B, a->L = L, a->D = D;
+  a->scale_dtype = scale_dtype, a->pos_dtype = pos_dtype, a->eps = eps;
+  a->pos = positions;
+  for (int i = 0; i < 3; ++i) a->pos_stride[i] = pos_strides[i];
+  a->t[0].scale = q_scale, a->t[1].scale = k_scale;
+  a->vec = 1;
+  return GFX_OK;
+}
+
+// One strided [B, H, L, D] array: copies its strides, checks its pointer, and clears a->vec where its rows are not
+// all 16-byte aligned.
+static int rope_array(const char* fn, const char* name, RopeArgs* a, int dtype, int H, const void* p,
+                      const int64_t* strides, long long (&to)[3]) {
+  if (H == 0 || (long long)a->B * a->L == 0) return GFX_OK;
+  if (!p || !strides) return set_error(GFX_ERR_INVALID, "%s: %s is a null pointer", fn, name);
+  const long long size = dtype == GFX_DTYPE_F32 ? 4 : 2;
+  if ((uintptr_t)p % size) return set_error(GFX_ERR_INVALID, "%s: %s is not aligned to its element size", fn, name);
+  const int n[3] = {a->B, H, a->L};
+  bool vec = ((uintptr_t)p & 15) == 0;
+  for (int i = 0; i < 3; ++i) {
+    to[i] = strides[i];
+    if (n[i] > 1 && (strides[i] * size) % 16 != 0) vec = false;
+  }
+  if (!vec) a->vec = 0;
+  return GFX_OK;
+}
+
+size_t qk_norm_rope_workspace_bytes(int D) { return D <= 0 ? 0 : (size_t)kRopeMaxBlocks * 2 * (size_t)D * sizeof(float); }
+
+int qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                 const void* positions, int pos_dtype, const int64_t* pos_strides, const void* q_scale,
+                 const void* k_scale, int scale_dtype, void* q_out, const int64_t* q_out_strides, void* k_out,
+                 const int64_t* k_out_strides, int B, int Hq, int Hk, int L, int D, const int* axes_dims, int n_axes,
+                 double theta, int interleaved, float eps, gfx_stream_t stream) {
+  const char* fn = "qk_norm_rope";
+  RopeArgs a;
+  int rc = rope_common(fn, &a, dtype, positions, pos_dtype, pos_strides, q_scale, k_scale, scale_dtype, B, Hq, Hk, L, D,
+                       axes_dims, n_axes, theta, interleaved, eps);
+  if (rc || (rc = rope_array(fn, "q", &a, dtype, Hq, q, q_strides, a.t[0].in_stride)) ||
+      (rc = rope_array(fn, "k", &a, dtype, Hk, k, k_strides, a.t[1].in_stride)) ||
+      (rc = rope_array(fn, "q_out", &a, dtype, Hq, q_out, q_out_strides, a.t[0].out_stride)) ||
+      (rc = rope_array(fn, "k_out", &a, dtype, Hk, k_out, k_out_strides, a.t[1].out_stride)))
+    return rc;
+  if ((long long)B * L == 0 || Hq + Hk == 0) return GFX_OK;
+  a.t[0].in = q, a.t[1].in = k, a.t[0].out = q_out, a.t[1].out = k_out;
+  return launch_rope(a, dtype, interleaved != 0, false, nullptr, nullptr, reinterpret_cast<cudaStream_t>(stream),
+                     sm_count(current_device()));
+}
+
+int qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                          const int64_t* dk_out_strides, const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, int dtype, const void* positions, int pos_dtype,
+                          const int64_t* pos_strides, const void* q_scale, const void* k_scale, int scale_dtype,
+                          void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dq_scale,
+                          void* dk_scale, int B, int Hq, int Hk, int L, int D, const int* axes_dims, int n_axes,
+                          double theta, int interleaved, float eps, void* workspace, size_t workspace_bytes,
+                          gfx_stream_t stream) {
+  const char* fn = "qk_norm_rope_backward";
+  RopeArgs a;
+  int rc = rope_common(fn, &a, dtype, positions, pos_dtype, pos_strides, q_scale, k_scale, scale_dtype, B, Hq, Hk, L, D,
+                       axes_dims, n_axes, theta, interleaved, eps);
+  if (rc || (rc = rope_array(fn, "dq_out", &a, dtype, Hq, dq_out, dq_out_strides, a.t[0].in_stride)) ||
+      (rc = rope_array(fn, "dk_out", &a, dtype, Hk, dk_out, dk_out_strides, a.t[1].in_stride)) ||
+      (rc = rope_array(fn, "dq", &a, dtype, Hq, dq, dq_strides, a.t[0].out_stride)) ||
+      (rc = rope_array(fn, "dk", &a, dtype, Hk, dk, dk_strides, a.t[1].out_stride)))
+    return rc;
+  if (q_scale && (rc = rope_array(fn, "q", &a, dtype, Hq, q, q_strides, a.t[0].x_stride))) return rc;
+  if (k_scale && (rc = rope_array(fn, "k", &a, dtype, Hk, k, k_strides, a.t[1].x_stride))) return rc;
+  if ((dq_scale && !q_scale) || (dk_scale && !k_scale))
+    return set_error(GFX_ERR_INVALID, "%s: a scale's gradient is asked for, but the scale is null", fn);
+  const uintptr_t es = scale_dtype == GFX_DTYPE_F32 ? 3 : 1;
+  if (((uintptr_t)dq_scale & es) || ((uintptr_t)dk_scale & es))
+    return set_error(GFX_ERR_INVALID, "%s: a scale's gradient is not aligned to its element size", fn);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dq_scale || dk_scale) {
+    if (!workspace || workspace_bytes < qk_norm_rope_workspace_bytes(D) || ((uintptr_t)workspace & 15))
+      return set_error(GFX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", fn,
+                       qk_norm_rope_workspace_bytes(D), workspace ? workspace_bytes : (size_t)0);
+    a.partial = static_cast<float*>(workspace);
+  }
+  if ((long long)B * L == 0 || Hq + Hk == 0) {  // no rows: the scales' gradients are zero
+    const size_t bytes = (size_t)D * (scale_dtype == GFX_DTYPE_F32 ? 4 : 2);
+    for (void* d : {dq_scale, dk_scale})
+      if (d && cudaMemsetAsync(d, 0, bytes, st) != cudaSuccess) return check_launch("cudaMemsetAsync");
+    return GFX_OK;
+  }
+  a.t[0].in = dq_out, a.t[1].in = dk_out, a.t[0].out = dq, a.t[1].out = dk;
+  a.t[0].x = q, a.t[1].x = k;
+  return launch_rope(a, dtype, interleaved != 0, true, dq_scale, dk_scale, st, sm_count(current_device()));
 }
 
 }  // extern "C"

@@ -90,6 +90,63 @@ int launch_attention(int qk_mode, int pv_mode, const void* q, const float* q_sca
                      const float* k_scale, const void* vt, const float* v_scale, const uint8_t* keep, void* out,
                      int B, int H, int KVH, int Lq, int Lk, float skip_below, cudaStream_t stream);
 
+// AdamW over many tensors -- adamw.cu
+constexpr int kAdamwMaxTensors = 56;  // per launch: the table travels in the kernel's arguments (4 KB)
+struct AdamwTensor {
+  void* p;
+  const void* g;
+  void* m;         // float32 values, or int8 codes
+  void* v;         // float32 values, or uint8 codes of the root
+  float* m_scale;  // 8-bit: one per 256 elements
+  float* v_scale;
+  long long n;
+  int first_cta;
+  int aligned;     // every array 16-byte aligned
+};
+struct AdamwScalars {
+  const float* grad_scale;  // device, or null: gradients are multiplied by it
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float decay;       // 1 - lr * weight_decay
+  float step_size;   // lr / (1 - beta1^t)
+  float root_scale;  // 1 / sqrt(1 - beta2^t)
+  float eps;
+};
+int launch_adamw(const AdamwTensor* tensors, int count, int p_dtype, int g_dtype, bool bits8, const AdamwScalars& c,
+                 cudaStream_t st, int sms);
+int launch_moment_values(const void* codes, const float* scale, float* out, long long n, int second, int vec,
+                         cudaStream_t st, int sms);
+
+// q/k normalisation with rotary positions -- rotary.cu
+constexpr int kRopeMaxDim = 256;
+constexpr int kRopeMaxAxes = 8;
+constexpr int kRopeMaxBlocks = 148 * 8;  // blocks of one launch; the backward's partial sums have this many rows
+enum : int { kPositionF32 = 0, kPositionI32 = 1, kPositionI64 = 2 };
+struct RopeTensor {
+  const void* in;   // forward: x; backward: dy          strides: batch, head, token (elements)
+  const void* x;    // backward: the forward's x (null without a scale)
+  void* out;        // forward: y; backward: dx
+  const void* scale;
+  long long in_stride[3], x_stride[3], out_stride[3];
+};
+struct RopeArgs {
+  RopeTensor t[2];  // q, k
+  int heads[2];
+  int B, L, D;
+  int pairs;        // rotated pairs
+  int scale_dtype, pos_dtype;
+  int vec;          // every row 16-byte aligned
+  int parts, steps_per_part;  // a token's heads in steps of 32 / lanes per row
+  float eps;
+  const void* pos;
+  long long pos_stride[3];  // batch, token, axis
+  float* partial;           // backward: [kRopeMaxBlocks][2][D], or null
+  double freq[kRopeMaxDim / 2];
+  unsigned char axis[kRopeMaxDim / 2];
+};
+void rope_frequencies(RopeArgs* a, const int* axes_dims, int n_axes, double theta);
+int launch_rope(RopeArgs& a, int dtype, bool pairs, bool backward, void* dq_scale, void* dk_scale, cudaStream_t st,
+                int sms);
+
 // loaders / helpers -- pack.cu
 int launch_int4_dequant(const void* wq, const void* ws, int scale_dtype, void* out, int out_dtype, int N, int K,
                         cudaStream_t stream, int qblock = 32);

@@ -1,0 +1,206 @@
+"""AdamW over many tensors in one launch, with moments in 32 or in 8 bits.
+
+The reference's training code (nodes/ComfyUI-Gfx906Int4/train_linear.py) leaves
+the optimizer to torch; these are the step a fine-tuning run takes here
+(csrc/adamw.cu behind the C ABI ``adamw_step``):
+
+  * ``AdamW``: a ``torch.optim.Optimizer`` over the functions below;
+  * ``adamw_step`` / ``adamw_step_8bit``: the step on plain tensor lists;
+  * ``moment_values``: what 8-bit moments stand for.
+
+8-bit moments: one float32 scale s for each 256 consecutive elements of a
+tensor. A first moment's code c in [-127, 127] stands for c |c| s. A second
+moment's code c in [0, 255] stands for (c^2 s)^2: its root is held, so that the
+ratio of the largest to the smallest held value is 255^4 within a block, and a
+positive second moment keeps at least the code 1.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib, ops
+
+BLOCK = 256  # elements that share one scale of an 8-bit moment
+
+
+def moment_scales(numel: int) -> int:
+    """Scales that an 8-bit moment of ``numel`` elements has."""
+    return -(-numel // BLOCK)
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _check_lists(params, groups):
+    for name, tensors in groups:
+        if len(tensors) != len(params):
+            raise RuntimeError(f"{name} has {len(tensors)} tensors, params {len(params)}")
+    if not params:
+        return
+    dev, dt, gt = params[0].device, params[0].dtype, groups[0][1][0].dtype
+    ops._dtype_code(dt)
+    ops._dtype_code(gt)
+    ops._require_cuda(params[0], "params[0]")
+    for i, p in enumerate(params):
+        if p.dtype != dt or p.device != dev or not p.is_contiguous():
+            raise RuntimeError(f"params[{i}] must be contiguous, {dt} on {dev} as params[0] is; got {p.dtype} on "
+                               f"{p.device}, strides {p.stride()}")
+
+
+def _check(name, tensors, params, dtype, numel):
+    dev = params[0].device if params else None
+    for i, t in enumerate(tensors):
+        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.numel() != numel(params[i]):
+            raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {numel(params[i])} elements; "
+                               f"got {t.dtype} on {t.device}, {tuple(t.shape)}, strides {t.stride()}")
+
+
+def _grad_scale(grad_scale, params):
+    if grad_scale is None:
+        return None
+    if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != params[0].device:
+        raise RuntimeError(f"grad_scale must be one float32 value on {params[0].device}, got {grad_scale.dtype} "
+                           f"{tuple(grad_scale.shape)} on {grad_scale.device}")
+    return grad_scale.data_ptr()
+
+
+def _call(params, grads, m, v, ms, vs, bits, step, lr, betas, eps, weight_decay, grad_scale):
+    n = len(params)
+    scale = _grad_scale(grad_scale, params)
+    numel = (ctypes.c_int64 * n)(*[p.numel() for p in params])
+    with torch.cuda.device(params[0].device):
+        _lib.call("adamw_step", _pointers(params), _pointers(grads), _pointers(m), _pointers(v),
+                  _pointers(ms) if bits == 8 else None, _pointers(vs) if bits == 8 else None, numel, n,
+                  ops._dtype_code(params[0].dtype), ops._dtype_code(grads[0].dtype), bits, int(step), float(lr),
+                  float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale,
+                  ops._stream(params[0].device))
+    torch.autograd.graph.increment_version(params)  # autograd sees the kernel's write as any in-place change
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None) -> None:
+    """One AdamW step in place on lists of tensors.
+
+    params: contiguous CUDA tensors of one dtype (float32 / float16 /
+    bfloat16); grads: the same shapes, one dtype; exp_avgs, exp_avg_sqs:
+    float32. ``step`` counts from 1. ``grad_scale`` (one float32 value on the
+    device) multiplies every gradient, for clipping or unscaling without a
+    pass of its own."""
+    _check_lists(params, [("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)])
+    if not params:
+        return
+    same = torch.Tensor.numel
+    _check("grads", grads, params, grads[0].dtype, same)
+    _check("exp_avgs", exp_avgs, params, torch.float32, same)
+    _check("exp_avg_sqs", exp_avg_sqs, params, torch.float32, same)
+    _call(params, grads, exp_avgs, exp_avg_sqs, None, None, 32, step, lr, betas, eps, weight_decay, grad_scale)
+
+
+def adamw_step_8bit(params, grads, m_codes, m_scales, v_codes, v_scales, *, step: int, lr: float, betas=(0.9, 0.999),
+                    eps: float = 1e-8, weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None) -> None:
+    """``adamw_step`` with moments in 8 bits: m_codes int8 and v_codes uint8
+    with a tensor's elements, m_scales and v_scales float32 with one value per
+    256 elements (``moment_scales``). Zeros are a fresh state. The parameters
+    move by the moments as computed, before they are rounded to codes."""
+    _check_lists(params, [("grads", grads), ("m_codes", m_codes), ("m_scales", m_scales), ("v_codes", v_codes),
+                          ("v_scales", v_scales)])
+    if not params:
+        return
+    same = torch.Tensor.numel
+
+    def scales(p):
+        return moment_scales(p.numel())
+
+    _check("grads", grads, params, grads[0].dtype, same)
+    _check("m_codes", m_codes, params, torch.int8, same)
+    _check("v_codes", v_codes, params, torch.uint8, same)
+    _check("m_scales", m_scales, params, torch.float32, scales)
+    _check("v_scales", v_scales, params, torch.float32, scales)
+    _call(params, grads, m_codes, v_codes, m_scales, v_scales, 8, step, lr, betas, eps, weight_decay, grad_scale)
+
+
+def moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The float32 values that 8-bit moments stand for, in codes' shape: int8
+    codes are a first moment's, uint8 codes a second's."""
+    ops._require_cuda(codes, "codes")
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise RuntimeError(f"codes must be int8 (first moment) or uint8 (second moment), got {codes.dtype}")
+    if scales.dtype != torch.float32 or scales.numel() != moment_scales(codes.numel()) or scales.device != codes.device:
+        raise RuntimeError(f"scales must be {moment_scales(codes.numel())} float32 values on {codes.device}, got "
+                           f"{scales.dtype} {tuple(scales.shape)} on {scales.device}")
+    c, s = codes.contiguous(), scales.contiguous()
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    with torch.cuda.device(codes.device):
+        _lib.call("adamw_moment_values", c.data_ptr(), s.data_ptr(), out.data_ptr(), c.numel(),
+                  int(codes.dtype == torch.uint8), ops._stream(codes.device))
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay on CUDA parameters; ``state_bits`` 32
+    or 8 chooses how both moments are held. Each group's parameters move in as
+    few launches as their number asks for (one per 56 tensors), separately for
+    each pair of parameter and gradient dtype. ``step(grad_scale=...)`` as
+    ``adamw_step``'s."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"expected lr, eps, weight_decay >= 0 and betas in [0, 1); got lr={lr} eps={eps} "
+                             f"weight_decay={weight_decay} betas={betas}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def _fresh(self, p: torch.Tensor, bits: int) -> dict:
+        if bits == 32:
+            return {"step": 0, "exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device),
+                    "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
+        n = moment_scales(p.numel())
+        return {"step": 0, "m_codes": torch.zeros(p.shape, dtype=torch.int8, device=p.device),
+                "m_scales": torch.zeros(n, dtype=torch.float32, device=p.device),
+                "v_codes": torch.zeros(p.shape, dtype=torch.uint8, device=p.device),
+                "v_scales": torch.zeros(n, dtype=torch.float32, device=p.device)}
+
+    def load_state_dict(self, state_dict):
+        """torch's loader casts a parameter's state to the parameter's dtype;
+        the moments keep their own."""
+        super().load_state_dict(state_dict)
+        index = {i: p for g, h in zip(state_dict["param_groups"], self.param_groups)
+                 for i, p in zip(g["params"], h["params"])}
+        for i, saved in state_dict["state"].items():
+            p = index[i]
+            self.state[p] = {k: (v.detach().clone().to(p.device) if torch.is_tensor(v) else v)
+                             for k, v in saved.items()}
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale: torch.Tensor | None = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            lists: dict = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW takes dense gradients")
+                st = self.state[p]
+                if not st:
+                    st.update(self._fresh(p, group["state_bits"]))
+                st["step"] += 1
+                lists.setdefault((p.device, p.dtype, p.grad.dtype, st["step"]), []).append((p, p.grad.contiguous(), st))
+            for (*_, step), items in lists.items():
+                ps, gs, sts = zip(*items)
+                more = dict(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                            weight_decay=group["weight_decay"], grad_scale=grad_scale)
+                if group["state_bits"] == 32:
+                    adamw_step(ps, gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts], **more)
+                else:
+                    adamw_step_8bit(ps, gs, *([s[k] for s in sts]
+                                              for k in ("m_codes", "m_scales", "v_codes", "v_scales")), **more)
+        return loss

@@ -316,6 +316,74 @@ int scales_to_f16(const float* scale, void* scale_f16, int64_t n, int* inexact, 
 int hadamard_rotate(const void* x, int x_dtype, const float* sign, void* out, int out_dtype, int64_t rows, int K,
                     int group, gfx_stream_t stream);
 
+/*
+ * One AdamW step (decoupled weight decay) over `count` tensors, in place:
+ *   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2,
+ *   p <- p (1 - lr wd) - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
+ * with g multiplied by *grad_scale first (a device float; NULL: 1). No
+ * counterpart in the reference, whose training code leaves the optimizer to
+ * torch.
+ *   p, g, m, v: host arrays of `count` device pointers; numel: elements of each
+ *   (0 allowed). p of p_dtype, g of g_dtype, one dtype for the whole list.
+ *   state_bits 32: m, v float32; m_scale, v_scale NULL.
+ *   state_bits 8:  m int8, v uint8, m_scale / v_scale host arrays of device
+ *   pointers to float32 scales, one per 256 consecutive elements (the last
+ *   block of a tensor may be short). A first-moment code c stands for
+ *   c |c| scale, a second-moment code for (c^2 scale)^2; all-zero codes and
+ *   scales are a fresh state. A block that met an infinite or NaN moment has a
+ *   NaN scale from then on.
+ * step counts from 1. Tensors may not overlap. The host arrays are read before
+ * the call returns.
+ */
+int adamw_step(void* const* p, const void* const* g, void* const* m, void* const* v, float* const* m_scale,
+               float* const* v_scale, const int64_t* numel, int count, int p_dtype, int g_dtype, int state_bits,
+               int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+               const float* grad_scale, gfx_stream_t stream);
+
+/* The float32 values that 8-bit moments stand for: codes int8 (second = 0) or
+ * uint8 (second = 1), [n], scale [ceil(n / 256)], out [n]. */
+int adamw_moment_values(const void* codes, const float* scale, float* out, int64_t n, int second, gfx_stream_t stream);
+
+/*
+ * RMS normalisation of q and k with multi-axis rotary positions (no kernel in
+ * the reference: its host framework's model does both in torch). Per row x of
+ * D elements: z = scale * x / sqrt(mean(x^2) + eps) where the tensor has a
+ * scale (else z = x), then pair p of axis a turned by the angle
+ * position[a] * theta^(-2 j / axes_dims[a]), j the pair's index within its
+ * axis; elements past sum(axes_dims) pass through.
+ *   q [B, Hq, L, D], k [B, Hk, L, D] (Hk may be 0, k NULL): strides in elements
+ *   of batch, head and token; the last dimension is contiguous. dtype 0/1/2.
+ *   positions: pos_dtype 0 float32 / 1 int32 / 2 int64, strides of batch,
+ *   token and axis (0 broadcasts).
+ *   axes_dims[n_axes]: even, n_axes in [1, 8], sum <= D.
+ *   interleaved 1: pairs (2p, 2p+1); 0: (p, p + sum/2), sum % 8 == 0.
+ *   q_scale, k_scale: [D] of scale_dtype, either may be NULL.
+ *   D % 8 == 0, D <= 256. Outputs [B, H, L, D] with their own strides; they
+ *   may not overlap an input.
+ */
+int qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                 const void* positions, int pos_dtype, const int64_t* pos_strides, const void* q_scale,
+                 const void* k_scale, int scale_dtype, void* q_out, const int64_t* q_out_strides, void* k_out,
+                 const int64_t* k_out_strides, int B, int Hq, int Hk, int L, int D, const int* axes_dims, int n_axes,
+                 double theta, int interleaved, float eps, gfx_stream_t stream);
+/*
+ * Its gradient: dq_out, dk_out are the outputs' gradients, q, k the forward's
+ * inputs (read only where the tensor has a scale; else may be NULL), dq, dk the
+ * results, dq_scale / dk_scale [D] of scale_dtype (NULL: not wanted). Scale
+ * gradients are summed in float32 in a fixed order through `workspace`
+ * (qk_norm_rope_workspace_bytes(D) bytes, 16-byte aligned, any contents;
+ * may be NULL when neither is wanted).
+ */
+int qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                          const int64_t* dk_out_strides, const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, int dtype, const void* positions, int pos_dtype,
+                          const int64_t* pos_strides, const void* q_scale, const void* k_scale, int scale_dtype,
+                          void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dq_scale,
+                          void* dk_scale, int B, int Hq, int Hk, int L, int D, const int* axes_dims, int n_axes,
+                          double theta, int interleaved, float eps, void* workspace, size_t workspace_bytes,
+                          gfx_stream_t stream);
+size_t qk_norm_rope_workspace_bytes(int D);
+
 #ifdef __cplusplus
 }
 #endif
