@@ -811,4 +811,83 @@ int qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, con
   return launch_rope(a, dtype, interleaved != 0, true, dq_scale, dk_scale, st, sm_count(current_device()));
 }
 
+static int gated_common(const char* fn, GatedArgs* a, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
+                        const void* w_up, int64_t ldu, int dtype, int act, int M, int K, int F) {
+  if (dtype != GFX_DTYPE_F16 && dtype != GFX_DTYPE_BF16)
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: dtype must be 1 (f16) or 2 (bf16), got %d", fn, dtype);
+  if (act < 0 || act > 2)
+    return set_error(GFX_ERR_INVALID, "%s: act must be 0 silu / 1 gelu / 2 gelu_tanh, got %d", fn, act);
+  if (M < 0 || K <= 0 || F <= 0 || K % 8 != 0 || F % 8 != 0)
+    return set_error(GFX_ERR_INVALID, "%s: expected M >= 0 and K, F positive multiples of 8; got M=%d K=%d F=%d", fn, M,
+                     K, F);
+  if (F > (1 << 22) || K > (1 << 22))
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: K and F go up to 2^22, got K=%d F=%d", fn, K, F);
+  if (ldx < K || ldg < K || ldu < K || ldx % 8 != 0 || ldg % 8 != 0 || ldu % 8 != 0)
+    return set_error(GFX_ERR_INVALID, "%s: row strides must be multiples of 8 and at least K, got x %lld gate %lld up "
+                     "%lld", fn, (long long)ldx, (long long)ldg, (long long)ldu);
+  *a = GatedArgs{x, w_gate, w_up, nullptr, nullptr, ldx, ldg, ldu, M, K, F};
+  return GFX_OK;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
+                 const void* b_gate, const void* b_up, int dtype, int act, void* h, float* save, int M, int K, int F,
+                 gfx_stream_t stream) {
+  const char* fn = "gated_linear";
+  GatedArgs a;
+  int rc = gated_common(fn, &a, x, ldx, w_gate, ldg, w_up, ldu, dtype, act, M, K, F);
+  if (rc) return rc;
+  if (M == 0) return GFX_OK;
+  if (!x || !w_gate || !w_up || !h) return set_error(GFX_ERR_INVALID, "%s: x, w_gate, w_up or h is a null pointer", fn);
+  if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(h) || !aligned16(save))
+    return set_error(GFX_ERR_INVALID, "%s: x, w_gate, w_up, h and save must be 16-byte aligned", fn);
+  if (((uintptr_t)b_gate & 1) || ((uintptr_t)b_up & 1))
+    return set_error(GFX_ERR_INVALID, "%s: a bias is not aligned to its element size", fn);
+  a.b_gate = b_gate, a.b_up = b_up;
+  const int dev = current_device();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if ((rc = check_device_health(fn, dev, nullptr, 0, st))) return rc;
+  return launch_gated_forward(a, dtype, act, h, save, st, sm_count(dev));
+}
+
+size_t gated_linear_backward_workspace_bytes(int M, int F) {
+  return M <= 0 || F <= 0 ? 0 : gated_backward_workspace(M, F);
+}
+
+int gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
+                          const void* w_up, int64_t ldu, const float* save, int dtype, int act, void* dx,
+                          void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int K, int F, void* workspace,
+                          size_t workspace_bytes, gfx_stream_t stream) {
+  const char* fn = "gated_linear_backward";
+  GatedArgs a;
+  int rc = gated_common(fn, &a, x, ldx, w_gate, ldg, w_up, ldu, dtype, act, M, K, F);
+  if (rc) return rc;
+  if (lddh < F || lddh % 8 != 0)
+    return set_error(GFX_ERR_INVALID, "%s: dh's row stride must be a multiple of 8 and at least F, got %lld", fn,
+                     (long long)lddh);
+  if (!aligned16(dh) || !aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(save) || !aligned16(dx) ||
+      !aligned16(dw_gate) || !aligned16(dw_up))
+    return set_error(GFX_ERR_INVALID, "%s: dh, x, w_gate, w_up, save, dx, dw_gate and dw_up must be 16-byte aligned", fn);
+  if (((uintptr_t)db_gate & 1) || ((uintptr_t)db_up & 1))
+    return set_error(GFX_ERR_INVALID, "%s: a bias gradient is not aligned to its element size", fn);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int dev = current_device();
+  if (M == 0) {  // no tokens: the weights' and biases' gradients are zero
+    for (void* d : {dw_gate, dw_up})
+      if (d && cudaMemsetAsync(d, 0, (size_t)F * K * 2, st) != cudaSuccess) return check_launch("cudaMemsetAsync");
+    for (void* d : {db_gate, db_up})
+      if (d && cudaMemsetAsync(d, 0, (size_t)F * 2, st) != cudaSuccess) return check_launch("cudaMemsetAsync");
+    return GFX_OK;
+  }
+  if (!dh || !save || ((dw_gate || dw_up) && !x) || (dx && (!w_gate || !w_up)))
+    return set_error(GFX_ERR_INVALID, "%s: dh, save, or an operand of a gradient that is asked for is a null pointer", fn);
+  if (!workspace || workspace_bytes < gated_backward_workspace(M, F) || !aligned16(workspace))
+    return set_error(GFX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", fn,
+                     gated_backward_workspace(M, F), workspace ? workspace_bytes : (size_t)0);
+  if ((rc = check_device_health(fn, dev, nullptr, 0, st))) return rc;
+  const GatedGrads d{dx, dw_gate, dw_up, db_gate, db_up};
+  return launch_gated_backward(a, dtype, act, dh, lddh, save, d, workspace, st, sm_count(dev));
+}
+
 }  // extern "C"

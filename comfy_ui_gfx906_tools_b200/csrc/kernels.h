@@ -147,6 +147,21 @@ void rope_frequencies(RopeArgs* a, const int* axes_dims, int n_axes, double thet
 int launch_rope(RopeArgs& a, int dtype, bool pairs, bool backward, void* dq_scale, void* dk_scale, cudaStream_t st,
                 int sms);
 
+// gated feed-forward product, h = a(x Wg^T + bg) * (x Wu^T + bu) -- gated.cu
+struct GatedArgs {
+  const void *x, *w_gate, *w_up, *b_gate, *b_up;  // biases may be null
+  long long ldx, ldg, ldu;                        // row strides (elements)
+  int M, K, F;
+};
+struct GatedGrads {  // null: not wanted
+  void *x, *w_gate, *w_up, *b_gate, *b_up;
+};
+// save: float32 [2][M][F] (g, then u), or null
+int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms);
+int launch_gated_backward(const GatedArgs& a, int dtype, int act, const void* dh, long long ldh, const float* save,
+                          const GatedGrads& d, void* workspace, cudaStream_t st, int sms);
+size_t gated_backward_workspace(int M, int F);
+
 // loaders / helpers -- pack.cu
 int launch_int4_dequant(const void* wq, const void* ws, int scale_dtype, void* out, int out_dtype, int N, int K,
                         cudaStream_t stream, int qblock = 32);

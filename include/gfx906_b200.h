@@ -384,6 +384,35 @@ int qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, con
                           gfx_stream_t stream);
 size_t qk_norm_rope_workspace_bytes(int D);
 
+/*
+ * Gated feed-forward product (no kernel in the reference, whose host
+ * framework's model does it as two linears, an activation and a product):
+ *   h = act(x Wg^T + bg) * (x Wu^T + bu)
+ *   x [M, K], w_gate / w_up [F, K], h [M, F]: dtype 1 (f16) or 2 (bf16), rows
+ *   contiguous, row strides ldx / ldg / ldu in elements (multiples of 8), h
+ *   dense; b_gate / b_up [F] of dtype, or NULL. K % 8 == 0, F % 8 == 0, all
+ *   arrays 16-byte aligned (biases: to their element).
+ *   act: 0 silu, 1 gelu (erf), 2 gelu with the tanh approximation.
+ *   save: float32 [2][M][F] that receives g and u for the backward, or NULL.
+ * Products accumulate in float32; h is rounded once.
+ */
+int gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
+                 const void* b_gate, const void* b_up, int dtype, int act, void* h, float* save, int M, int K, int F,
+                 gfx_stream_t stream);
+/*
+ * Its gradients from dh [M, F] (row stride lddh, a multiple of 8) and the
+ * forward's save:
+ *   dx [M, K], dw_gate / dw_up [F, K], db_gate / db_up [F], dense, of dtype;
+ *   each may be NULL (not computed). x is read only for the weights' gradients.
+ * workspace: gated_linear_backward_workspace_bytes(M, F) bytes, 16-byte
+ * aligned, any contents.
+ */
+int gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
+                          const void* w_up, int64_t ldu, const float* save, int dtype, int act, void* dx,
+                          void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int K, int F, void* workspace,
+                          size_t workspace_bytes, gfx_stream_t stream);
+size_t gated_linear_backward_workspace_bytes(int M, int F);
+
 #ifdef __cplusplus
 }
 #endif

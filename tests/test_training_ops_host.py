@@ -78,3 +78,37 @@ def test_rope_backward_checks(built_lib):
     assert _rope(built_lib, False, B=0, q=None, k=None, pos=None) == _lib.GFX_OK
     assert _rope(built_lib, False, Hq=0, Hk=0) == _lib.GFX_OK
     assert _rope(built_lib, True, L=0, dqs=None, qs=None) == _lib.GFX_OK
+
+
+def _gated(lib, back=False, x=16, wg=16, wu=16, h=16, save=16, bg=None, dt=2, act=0, M=3, K=64, F=72, ldx=64, ldg=64,
+           ldu=64, lddh=72, ws=16, wsb=1 << 20, dx=16, dw=16):
+    if not back:
+        return lib.gated_linear(x, ldx, wg, ldg, wu, ldu, bg, None, dt, act, h, save, M, K, F, None)
+    return lib.gated_linear_backward(h, lddh, x, ldx, wg, ldg, wu, ldu, save, dt, act, dx, dw, None, bg, None, M, K, F,
+                                     ws, wsb, None)
+
+
+@pytest.mark.parametrize("kw,code,needle", [
+    (dict(dt=0), UNSUPPORTED, "dtype"), (dict(act=3), INVALID, "act"), (dict(M=-1), INVALID, "M >= 0"),
+    (dict(K=60), INVALID, "multiples of 8"), (dict(F=70), INVALID, "multiples of 8"), (dict(K=0), INVALID, "K=0"),
+    (dict(F=1 << 23), UNSUPPORTED, "2^22"), (dict(ldx=56), INVALID, "row strides"), (dict(ldg=65), INVALID, "row strides"),
+    (dict(x=None), INVALID, "null"), (dict(wu=None), INVALID, "null"), (dict(h=None), INVALID, "null"),
+    (dict(x=24), INVALID, "16-byte"), (dict(h=8), INVALID, "16-byte"), (dict(save=4), INVALID, "16-byte"),
+    (dict(bg=17), INVALID, "bias"),
+])
+def test_gated_argument_checks(built_lib, kw, code, needle):
+    for back in (False, True):
+        assert _gated(built_lib, back, **kw) == code
+        assert needle in _lib.last_error()
+
+
+def test_gated_backward_checks(built_lib):
+    assert _gated(built_lib, True, lddh=64) == INVALID and "dh's row stride" in _lib.last_error()
+    assert _gated(built_lib, True, save=None) == INVALID
+    assert _gated(built_lib, True, dx=18) == INVALID
+    assert _gated(built_lib, True, ws=None) == WORKSPACE
+    assert _gated(built_lib, True, ws=24) == WORKSPACE
+    assert _gated(built_lib, True, wsb=100) == WORKSPACE and "workspace of" in _lib.last_error()
+    assert _gated(built_lib, False, M=0, x=None, h=None) == _lib.GFX_OK
+    assert _gated(built_lib, True, M=0, dx=None, dw=None, x=None) == _lib.GFX_OK
+    assert built_lib.gated_linear_backward_workspace_bytes(0, 8) == 0
