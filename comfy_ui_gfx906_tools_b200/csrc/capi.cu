@@ -243,8 +243,8 @@ int gfx_device_status(int clear) {
   int v = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return -set_error(GFX_ERR_CUDA, "gfx_device_status: %s", cudaGetErrorString(e));
-  const int parts[5] = {smallm_device_status(clear), tc_device_status(clear), selftest_device_status(clear),
-                         w4a4x_device_status(clear), attn_tc_device_status(clear)};
+  const int parts[6] = {smallm_device_status(clear), tc_device_status(clear), selftest_device_status(clear),
+                         w4a4x_device_status(clear), attn_tc_device_status(clear), gated_tc_device_status(clear)};
   for (int p : parts) {
     if (p < 0) return -set_error(GFX_ERR_CUDA, "gfx_device_status: reading a status word failed");
     if (p && !v) v = p;
@@ -820,8 +820,8 @@ static int gated_common(const char* fn, GatedArgs* a, const void* x, int64_t ldx
   if (M < 0 || K <= 0 || F <= 0 || K % 8 != 0 || F % 8 != 0)
     return set_error(GFX_ERR_INVALID, "%s: expected M >= 0 and K, F positive multiples of 8; got M=%d K=%d F=%d", fn, M,
                      K, F);
-  if (F > (1 << 22) || K > (1 << 22))
-    return set_error(GFX_ERR_UNSUPPORTED, "%s: K and F go up to 2^22, got K=%d F=%d", fn, K, F);
+  if (F > (1 << 22) || K > (1 << 22) || M > (1 << 30))
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: K and F go up to 2^22 and M to 2^30, got M=%d K=%d F=%d", fn, M, K, F);
   if (ldx < K || ldg < K || ldu < K || ldx % 8 != 0 || ldg % 8 != 0 || ldu % 8 != 0)
     return set_error(GFX_ERR_INVALID, "%s: row strides must be multiples of 8 and at least K, got x %lld gate %lld up "
                      "%lld", fn, (long long)ldx, (long long)ldg, (long long)ldu);

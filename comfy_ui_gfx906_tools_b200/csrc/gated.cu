@@ -9,85 +9,14 @@
 // roundings into every gradient, which nearly doubles its error (1.8 instead
 // of 1.4 times one rounding). dg and du are rounded to the inputs' type once,
 // because the tensor cores multiply 16-bit operands.
+#include <type_traits>
+
 #include "common.cuh"
 #include "gated.cuh"
 #include "kernels.h"
 
 namespace gfx {
 namespace gated {
-
-// ---------------------------------------------------------------------------
-// C[i, j] = sum over segments s and k of A_s[i, k] B_s[j, k], any strides: 64 x 64 tiles, 4 x 4 a thread
-// ---------------------------------------------------------------------------
-template <typename T>
-struct Operand {
-  const T* p;
-  long long row, k;  // strides
-};
-
-constexpr int kTile = 64, kDeep = 16;
-
-template <typename T>
-__device__ __forceinline__ void load_tile(float (*s)[kTile + 1], const Operand<T>& o, int i0, int rows, int k0, int K) {
-  for (int e = threadIdx.x; e < kTile * kDeep; e += 256) {
-    const int i = e / kDeep, k = e % kDeep;
-    s[k][i] = i0 + i < rows && k0 + k < K ? to_f32<T>(o.p[(i0 + i) * o.row + (k0 + k) * o.k]) : 0.0f;
-  }
-}
-
-// acc += A B^T over k < K
-template <typename T>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], float (*sa)[kTile + 1], float (*sb)[kTile + 1],
-                                             const Operand<T>& a, const Operand<T>& b, int i0, int I, int j0, int J,
-                                             int K) {
-  const int ti = threadIdx.x / 16 * 4, tj = threadIdx.x % 16 * 4;
-  for (int k0 = 0; k0 < K; k0 += kDeep) {
-    __syncthreads();
-    load_tile<T>(sa, a, i0, I, k0, K);
-    load_tile<T>(sb, b, j0, J, k0, K);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-      for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[y][x] += sa[k][ti + y] * sb[k][tj + x];
-  }
-}
-
-template <typename T, int kAct>
-__global__ void __launch_bounds__(256) forward_kernel(Operand<T> x, Operand<T> wg, Operand<T> wu, const T* bg,
-                                                      const T* bu, T* h, float* save, int M, int K, int F) {
-  __shared__ float sa[kDeep][kTile + 1], sb[kDeep][kTile + 1];
-  const int i0 = blockIdx.y * kTile, j0 = blockIdx.x * kTile;
-  float g[4][4] = {}, u[4][4] = {};
-  tile_product<T>(g, sa, sb, x, wg, i0, M, j0, F, K);
-  tile_product<T>(u, sa, sb, x, wu, i0, M, j0, F, K);
-  const int ti = i0 + threadIdx.x / 16 * 4, tj = j0 + threadIdx.x % 16 * 4;
-  for (int y = 0; y < 4; ++y)
-    for (int c = 0; c < 4; ++c) {
-      const long long i = ti + y;
-      const int j = tj + c;
-      if (i >= M || j >= F) continue;
-      const float gv = g[y][c] + (bg ? to_f32<T>(bg[j]) : 0.0f), uv = u[y][c] + (bu ? to_f32<T>(bu[j]) : 0.0f);
-      h[i * F + j] = from_f32<T>(activation<kAct>(gv) * uv);
-      if (save) save[i * F + j] = gv, save[(long long)M * F + i * F + j] = uv;
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(Operand<T> a0, Operand<T> b0, Operand<T> a1, Operand<T> b1,
-                                                      int segments, T* c, int I, int J, int K) {
-  __shared__ float sa[kDeep][kTile + 1], sb[kDeep][kTile + 1];
-  const int i0 = blockIdx.y * kTile, j0 = blockIdx.x * kTile;
-  float acc[4][4] = {};
-  tile_product<T>(acc, sa, sb, a0, b0, i0, I, j0, J, K);
-  if (segments == 2) tile_product<T>(acc, sa, sb, a1, b1, i0, I, j0, J, K);
-  const int ti = i0 + threadIdx.x / 16 * 4, tj = j0 + threadIdx.x % 16 * 4;
-  for (int y = 0; y < 4; ++y)
-    for (int x = 0; x < 4; ++x)
-      if (ti + y < I && tj + x < J) c[(long long)(ti + y) * J + tj + x] = from_f32<T>(acc[y][x]);
-}
 
 // ---------------------------------------------------------------------------
 // dg, du (one row of dgu [M, 2F]: dg then du) and, per block of rows, their column sums
@@ -160,32 +89,13 @@ size_t gated_backward_workspace(int M, int F) {
   return align_up((size_t)M * 2 * F * 2, 256) + (size_t)row_blocks(M) * 2 * F * sizeof(float);
 }
 
-template <typename T>
-static int gated_forward_t(const GatedArgs& a, int act, void* h, float* save, cudaStream_t st) {
-  using O = gated::Operand<T>;
-  const O x{(const T*)a.x, a.ldx, 1}, wg{(const T*)a.w_gate, a.ldg, 1}, wu{(const T*)a.w_up, a.ldu, 1};
-  const dim3 grid((a.F + gated::kTile - 1) / gated::kTile, (a.M + gated::kTile - 1) / gated::kTile);
-  auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, st>>>(x, wg, wu, (const T*)a.b_gate, (const T*)a.b_up, (T*)h, save, a.M, a.K, a.F);
-  };
-  if (act == gated::kSilu)
-    go(gated::forward_kernel<T, gated::kSilu>);
-  else if (act == gated::kGelu)
-    go(gated::forward_kernel<T, gated::kGelu>);
-  else
-    go(gated::forward_kernel<T, gated::kGeluTanh>);
-  return check_launch("gated forward_kernel");
-}
-
 int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms) {
-  (void)sms;
-  return dtype == GFX_DTYPE_F16 ? gated_forward_t<__half>(a, act, h, save, st)
-                                : gated_forward_t<__nv_bfloat16>(a, act, h, save, st);
+  return launch_gated_forward_tc(a, dtype, act, h, save, st, sms);
 }
 
 template <typename T>
 static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long long ldh, const float* save,
-                            const GatedGrads& d, void* workspace, cudaStream_t st) {
+                            const GatedGrads& d, void* workspace, cudaStream_t st, int sms) {
   T* dgu = static_cast<T*>(workspace);
   float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up((size_t)a.M * 2 * a.F * 2, 256));
   const int blocks = row_blocks(a.M);
@@ -206,31 +116,16 @@ static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long lo
     gated::bias_grad_kernel<T><<<(2 * a.F + 255) / 256, 256, 0, st>>>(partial, blocks, a.F, (T*)d.b_gate, (T*)d.b_up);
     if ((rc = check_launch("bias_grad_kernel"))) return rc;
   }
-  using O = gated::Operand<T>;
-  const int t = gated::kTile;
-  const long long F = a.F;
-  if (d.x) {  // dx = dg Wg + du Wu
-    gated::product_kernel<T><<<dim3((a.K + t - 1) / t, (a.M + t - 1) / t), 256, 0, st>>>(
-        O{dgu, 2 * F, 1}, O{(const T*)a.w_gate, 1, a.ldg}, O{dgu + F, 2 * F, 1}, O{(const T*)a.w_up, 1, a.ldu}, 2,
-        (T*)d.x, a.M, a.K, a.F);
-    if ((rc = check_launch("gated product_kernel"))) return rc;
-  }
-  for (int w = 0; w < 2; ++w) {  // dW = d^T x
-    T* out = (T*)(w ? d.w_up : d.w_gate);
-    if (!out) continue;
-    const O A{dgu + w * F, 1, 2 * F}, B{(const T*)a.x, 1, a.ldx};
-    gated::product_kernel<T><<<dim3((a.K + t - 1) / t, (a.F + t - 1) / t), 256, 0, st>>>(A, B, A, B, 1, out, a.F, a.K,
-                                                                                         a.M);
-    if ((rc = check_launch("gated product_kernel"))) return rc;
-  }
+  constexpr int kDtype = std::is_same<T, __half>::value ? GFX_DTYPE_F16 : GFX_DTYPE_BF16;
+  if (d.x && (rc = launch_gated_input_grad(a, kDtype, dgu, d.x, st, sms))) return rc;
+  if (d.w_gate || d.w_up) return launch_gated_weight_grad(a, kDtype, dgu, d.w_gate, d.w_up, st, sms);
   return GFX_OK;
 }
 
 int launch_gated_backward(const GatedArgs& a, int dtype, int act, const void* dh, long long ldh, const float* save,
                           const GatedGrads& d, void* workspace, cudaStream_t st, int sms) {
-  (void)sms;
-  return dtype == GFX_DTYPE_F16 ? gated_backward_t<__half>(a, act, dh, ldh, save, d, workspace, st)
-                                : gated_backward_t<__nv_bfloat16>(a, act, dh, ldh, save, d, workspace, st);
+  return dtype == GFX_DTYPE_F16 ? gated_backward_t<__half>(a, act, dh, ldh, save, d, workspace, st, sms)
+                                : gated_backward_t<__nv_bfloat16>(a, act, dh, ldh, save, d, workspace, st, sms);
 }
 
 }  // namespace gfx

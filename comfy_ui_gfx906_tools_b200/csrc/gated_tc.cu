@@ -1,0 +1,477 @@
+// The matrix products of the gated feed-forward block on the 5th-generation
+// tensor cores: forward (two projections, activation and product in one
+// kernel), input gradient and weight gradients.
+//
+//   forward  D[m, c] = sum_k x[m, k] W[c, k], c < 128 of the gate's rows, the
+//            other 128 of the up projection's same rows; the epilogue adds the
+//            biases and writes h = a(g) u (and g, u in float32 for a backward)
+//   dx       D[m, n] = sum_f dg[m, f] Wg[f, n] + sum_f du[m, f] Wu[f, n]
+//   dW       D[f, n] = sum_m dg[m, f] x[m, n]   (du for the up projection)
+//
+// One kernel with three roles. A cluster of two CTAs computes a 256 x 256 tile
+// with tcgen05.mma.cta_group::2 (M = 256, N = 256, K = 16): each CTA loads its
+// own 128 rows of A and its own 128 of the 256 columns of B, so an SM reads
+// 8 KB of shared memory per instruction instead of the 12 KB of a lone CTA's
+// 128 x 256 tile. In the forward CTA 0's half of B is the gate's weights and
+// CTA 1's the up projection's, so both projections of a feature land in the
+// same thread's TMEM lane. The operands that a gradient needs transposed (Wg
+// as [F, n], dg as [m, F], x as [m, n]) are read where they lie: TMA brings
+// 64 x 64 boxes and the descriptor names them MN-major.
+//
+// Per CTA: warp 8 loads (TMA, 7 stages of 32 KB), warp 9 of CTA 0 issues the
+// MMAs of the pair, warps 0-7 write tiles out (two 256-column accumulators in
+// TMEM, so a tile is written while the next one is multiplied): a thread owns
+// one row, and stores 32 bytes at a time, whole sectors, straight from
+// registers. A stage's barrier lives in CTA 0 and counts both CTAs' bytes.
+// Persistent: one pair per two SMs; tiles are walked in panels whose reused
+// operand stays in L2.
+#include <string.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "gated.cuh"
+#include "kernels.h"
+#include "tcgen05.cuh"
+
+namespace gfx {
+
+GFX_DEFINE_STATUS_READER(gated_tc_device_status)
+
+namespace gated {
+
+enum : int { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
+
+constexpr int kTileRows = 256, kTileCols = 256;  // of a pair; a CTA owns 128 rows
+constexpr int kStageK = 64, kStages = 7;
+constexpr int kOperandBytes = 128 * kStageK * 2;  // a CTA's half of A or of B per stage
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kEpilogueWarps = 8, kLoadWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 256;
+static_assert(kSmemBytes <= 232448, "shared memory");
+
+struct TcArgs {
+  CUtensorMap a0, a1, b0, b1;
+  int rows, cols;       // of the output (forward: M, F; dx: M, K; dW: F, K)
+  int depth;            // of the contraction, per segment (K; F; M)
+  int tiles_i, tiles_j; // row tiles and column tiles
+  int tiles_half;       // dW: row tiles of one weight; the second's follow
+  int panel;            // tiles of the fast direction that are walked before the slow one moves
+  int i_fast;
+  void* out0;           // h; dx; dWg
+  void* out1;           // dWu
+  long long ld;         // row stride of the outputs
+  const void* bias0;    // forward: bg, bu
+  const void* bias1;
+  float* save;          // forward: g, u
+  int wide;             // rows of every output are 32-byte aligned
+  int* status_host;
+};
+
+// TMA load of one box into this CTA, counted on the barrier at `bar`, which may be the other CTA's.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// Shared-memory descriptor of an MN-major operand in 64 (MN) x 64 (K) boxes with the 128-byte swizzle: 64 elements of
+// MN are 8 KB apart, 8 steps of K 1 KB.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <typename T, int kRole>
+constexpr uint32_t instruction_desc() {
+  const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  const uint32_t a_mn = kRole == kWeightGrad ? 1u : 0u, b_mn = kRole == kForward ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | (a_mn << 15) | (b_mn << 16) | ((uint32_t)(kTileCols >> 3) << 17) |
+         ((uint32_t)(kTileRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void st_global_v4(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// 32 consecutive values of one row from column c on; columns past `cols` (a multiple of 8) are left out.
+template <typename T>
+__device__ __forceinline__ void store_row(T* row, int c, int cols, bool wide, const float (&f)[32]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int q = 0; q < 32; q += 8) {
+      if (c + q >= cols) break;
+      uint32_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(f[q + j]);
+      if (wide) {
+        st_global_v8(row + c + q, v);
+      } else {
+        st_global_v4(row + c + q, v[0], v[1], v[2], v[3]);
+        st_global_v4(row + c + q + 4, v[4], v[5], v[6], v[7]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; q += 16) {
+      uint32_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = pack2<T>(f[q + 2 * j], f[q + 2 * j + 1]);
+      if (wide && c + q + 16 <= cols) {
+        st_global_v8(row + c + q, v);
+      } else {
+        if (c + q < cols) st_global_v4(row + c + q, v[0], v[1], v[2], v[3]);
+        if (c + q + 8 < cols) st_global_v4(row + c + q + 8, v[4], v[5], v[6], v[7]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void tile_at(const TcArgs& a, int t, int& i, int& j) {
+  const int nf = a.i_fast ? a.tiles_i : a.tiles_j, ns = a.i_fast ? a.tiles_j : a.tiles_i;
+  const int p = t / (a.panel * ns), rest = t - p * a.panel * ns;
+  const int width = min(a.panel, nf - p * a.panel);
+  const int f = p * a.panel + rest % width, s = rest / width;
+  i = a.i_fast ? f : s;
+  j = a.i_fast ? s : f;
+}
+
+template <typename T, int kRole, int kAct>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ TcArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * kStageBytes);  // CTA 0's: both CTAs' loads landed
+  uint64_t* empty = full + kStages;      // each CTA's: the MMAs have read the stage
+  uint64_t* acc_full = empty + kStages;  // each CTA's [2]: the accumulator is complete
+  uint64_t* acc_empty = acc_full + 2;    // CTA 0's [2]: both CTAs' epilogues are done with it
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cr = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = a.tiles_i * a.tiles_j;
+  const int segments = kRole == kInputGrad ? 2 : 1;
+  const int steps = (a.depth + kStageK - 1) / kStageK;  // per segment
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 2 * kEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc<2>(tmem_base, 512);
+  tc::tc_fence_before();
+  cluster_sync_all();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_base;
+
+  bool ok = true;
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      tma_prefetch_desc(&a.a0);
+      tma_prefetch_desc(&a.b0);
+      uint32_t it = 0;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int i, j;
+        tile_at(a, t, i, j);
+        const int half = kRole == kWeightGrad && i >= a.tiles_half;
+        const int r0 = (half ? i - a.tiles_half : i) * kTileRows + (int)cr * 128;
+        const int c0 = kRole == kForward ? j * 128 : j * kTileCols + (int)cr * 128;
+        for (int seg = 0; seg < segments && ok; ++seg) {
+          const CUtensorMap* am = (kRole == kWeightGrad ? half : seg) ? &a.a1 : &a.a0;
+          const CUtensorMap* bm = (kRole == kForward ? (int)cr : kRole == kInputGrad ? seg : 0) ? &a.b1 : &a.b0;
+          for (int k = 0; k < steps; ++k, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1, kDevErrEmptyBarrierTimeout)) {
+              ok = false;
+              break;
+            }
+            if (cr == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+            const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperandBytes;
+            const int kk = k * kStageK;
+            if constexpr (kRole == kWeightGrad) {
+              load_box(sa, am, bar, r0, kk);
+              load_box(sa + 8192, am, bar, r0 + 64, kk);
+            } else {
+              load_box(sa, am, bar, kk, r0);
+            }
+            if constexpr (kRole == kForward) {
+              load_box(sb, bm, bar, kk, c0);
+            } else {
+              load_box(sb, bm, bar, c0, kk);
+              load_box(sb + 8192, bm, bar, c0 + 64, kk);
+            }
+          }
+        }
+      }
+      if (!ok) {  // a wait gave up: let the copies in flight land before the memory is given back
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (cr == 0) {
+      constexpr uint32_t kId = instruction_desc<T, kRole>();
+      constexpr uint64_t kStepA = kRole == kWeightGrad ? 128 : 2, kStepB = kRole == kForward ? 2 : 128;  // 16 of K
+      uint32_t it = 0;
+      int n = 0;
+      for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+        const int acc = n & 1;
+        if (!mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1, kDevErrMmaBarrierTimeout)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const int total = steps * segments;
+        for (int k = 0; k < total; ++k, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&full[s], (it / kStages) & 1, kDevErrFullBarrierTimeout)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          if (lane == 0) {
+            const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperandBytes;
+            const uint64_t ad = kRole == kWeightGrad ? mn_desc(sa) : tc::sw128_desc(sa);
+            const uint64_t bd = kRole == kForward ? tc::sw128_desc(sb) : mn_desc(sb);
+#pragma unroll
+            for (int q = 0; q < kStageK / 16; ++q)
+              tc::umma_f16<2>(tmem + acc * kTileCols, ad + q * kStepA, bd + q * kStepB, kId, (k | q) != 0);
+            tc::umma_commit<2>(&empty[s], 0);
+            tc::umma_commit<2>(&empty[s], 1);
+            if (k == total - 1) {
+              tc::umma_commit<2>(&acc_full[acc], 0);
+              tc::umma_commit<2>(&acc_full[acc], 1);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if (lane == 0) {
+        tc::umma_commit<2>(drain, 0);
+        tc::umma_commit<2>(drain, 1);
+      }
+      __syncwarp();
+    }
+    if (!mbar_wait(drain, 0, kDevErrMmaBarrierTimeout)) ok = false;
+  } else {
+    const int quadrant = warp & 3, side = warp >> 2;  // 32 TMEM lanes; which half of the columns
+    const uint32_t lanes = tmem + ((uint32_t)(quadrant * 32) << 16);
+    int n = 0;
+    for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+      int i, j;
+      tile_at(a, t, i, j);
+      const int acc = n & 1;
+      const int half = kRole == kWeightGrad && i >= a.tiles_half;
+      const int row = (half ? i - a.tiles_half : i) * kTileRows + (int)cr * 128 + quadrant * 32 + lane;
+      if (!mbar_wait(&acc_full[acc], (n >> 1) & 1, kDevErrEpilogueBarrierTimeout)) {
+        ok = false;
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t d = lanes + acc * kTileCols;
+      if constexpr (kRole == kForward) {
+#pragma unroll 1
+        for (int c = side * 64; c < side * 64 + 64; c += 32) {
+          const int col = j * 128 + c;
+          if (col >= a.cols) break;
+          uint32_t gr[32], ur[32];
+          tc::tmem_ld32(d + c, gr);
+          tc::tmem_ld32(d + 128 + c, ur);
+          float g[32], u[32];
+          float bg = 0.0f, bu = 0.0f;
+          if (a.bias0 != nullptr && col + lane < a.cols) bg = to_f32<T>(static_cast<const T*>(a.bias0)[col + lane]);
+          if (a.bias1 != nullptr && col + lane < a.cols) bu = to_f32<T>(static_cast<const T*>(a.bias1)[col + lane]);
+#pragma unroll
+          for (int q = 0; q < 32; ++q) {
+            g[q] = __uint_as_float(gr[q]) + __shfl_sync(0xFFFFFFFFu, bg, q);
+            u[q] = __uint_as_float(ur[q]) + __shfl_sync(0xFFFFFFFFu, bu, q);
+          }
+          if (row < a.rows) {
+            if (a.save != nullptr) {
+              store_row<float>(a.save + (long long)row * a.cols, col, a.cols, a.wide, g);
+              store_row<float>(a.save + ((long long)a.rows + row) * a.cols, col, a.cols, a.wide, u);
+            }
+#pragma unroll
+            for (int q = 0; q < 32; ++q) g[q] = activation<kAct>(g[q]) * u[q];
+            store_row<T>(static_cast<T*>(a.out0) + row * a.ld, col, a.cols, a.wide, g);
+          }
+        }
+      } else {
+        T* out = static_cast<T*>(half ? a.out1 : a.out0) + row * a.ld;
+#pragma unroll 1
+        for (int c = side * 128; c < side * 128 + 128; c += 32) {
+          const int col = j * kTileCols + c;
+          if (col >= a.cols) break;
+          uint32_t v[32];
+          tc::tmem_ld32(d + c, v);
+          float f[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) f[q] = __uint_as_float(v[q]);
+          if (row < a.rows) store_row<T>(out, col, a.cols, a.wide, f);
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(&acc_empty[acc], 0);
+    }
+  }
+  if (!ok) mirror_device_error(a.status_host);
+  tc::tc_fence_before();
+  cluster_sync_all();  // no CTA leaves while its peer may still signal its barriers
+  tc::tc_fence_after();
+  if (warp == kMmaWarp) tc::tmem_dealloc<2>(tmem, 512);
+}
+
+template <typename T, int kRole, int kAct>
+static int launch_pair(TcArgs& a, cudaStream_t st, int sms) {
+  auto kern = pair_kernel<T, kRole, kAct>;
+  static int pairs_at_once[64] = {0};  // per device; every thread writes the same value
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return set_error(GFX_ERR_CUDA, "gated pair_kernel: no current device");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (pairs_at_once[dev] == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    int n = 0;
+    cfg.gridDim = dim3(sms / 2 * 2);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+    if (e != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      return set_error(GFX_ERR_CUDA, "gated pair_kernel: no CTA pair fits the GPU: %s", cudaGetErrorString(e));
+    }
+    pairs_at_once[dev] = n < sms / 2 ? n : sms / 2;
+  }
+  const int tiles = a.tiles_i * a.tiles_j;
+  cfg.gridDim = dim3(2 * (tiles < pairs_at_once[dev] ? tiles : pairs_at_once[dev]));
+  a.status_host = host_status_word(dev);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return set_error(GFX_ERR_CUDA, "gated pair_kernel launch: %s", cudaGetErrorString(e));
+  return check_launch("gated pair_kernel");
+}
+
+template <typename T>
+constexpr CUtensorMapDataType map_type() {
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// Boxes of 64 (inner) x `outer_box`, 128-byte swizzle.
+template <typename T>
+static int box_map(CUtensorMap* m, const void* p, long long inner, long long outer, long long ld, int outer_box) {
+  return make_tmap_2d(m, map_type<T>(), p, (uint64_t)inner, (uint64_t)outer, (uint64_t)ld * 2, 64, outer_box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static bool rows32(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0 && ld % 16 == 0; }
+
+template <typename T>
+static int forward_tc(const GatedArgs& g, int act, void* h, float* save, cudaStream_t st, int sms) {
+  TcArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc;
+  if ((rc = box_map<T>(&a.a0, g.x, g.K, g.M, g.ldx, 128)) || (rc = box_map<T>(&a.b0, g.w_gate, g.K, g.F, g.ldg, 128)) ||
+      (rc = box_map<T>(&a.b1, g.w_up, g.K, g.F, g.ldu, 128)))
+    return rc;
+  a.rows = g.M, a.cols = g.F, a.depth = g.K;
+  a.tiles_i = (g.M + 255) / 256, a.tiles_j = (g.F + 127) / 128;
+  a.panel = 16, a.i_fast = 1;
+  a.out0 = h, a.ld = g.F, a.bias0 = g.b_gate, a.bias1 = g.b_up, a.save = save;
+  a.wide = rows32(h, g.F) && (reinterpret_cast<uintptr_t>(save) & 31) == 0;
+  if (act == kSilu) return launch_pair<T, kForward, kSilu>(a, st, sms);
+  if (act == kGelu) return launch_pair<T, kForward, kGelu>(a, st, sms);
+  return launch_pair<T, kForward, kGeluTanh>(a, st, sms);
+}
+
+// dx [M, K] from dgu [M, 2F]
+template <typename T>
+static int input_grad_tc(const GatedArgs& g, const void* dgu, void* dx, cudaStream_t st, int sms) {
+  TcArgs a;
+  memset(&a, 0, sizeof(a));
+  const T* d = static_cast<const T*>(dgu);
+  int rc;
+  if ((rc = box_map<T>(&a.a0, d, g.F, g.M, 2ll * g.F, 128)) || (rc = box_map<T>(&a.a1, d + g.F, g.F, g.M, 2ll * g.F, 128)) ||
+      (rc = box_map<T>(&a.b0, g.w_gate, g.K, g.F, g.ldg, 64)) || (rc = box_map<T>(&a.b1, g.w_up, g.K, g.F, g.ldu, 64)))
+    return rc;
+  a.rows = g.M, a.cols = g.K, a.depth = g.F;
+  a.tiles_i = (g.M + 255) / 256, a.tiles_j = (g.K + 255) / 256;
+  a.panel = 16, a.i_fast = 1;
+  a.out0 = dx, a.ld = g.K;
+  a.wide = rows32(dx, g.K);
+  return launch_pair<T, kInputGrad, kSilu>(a, st, sms);
+}
+
+// dWg, dWu [F, K]: both, or one of them
+template <typename T>
+static int weight_grad_tc(const GatedArgs& g, const void* dgu, void* dwg, void* dwu, cudaStream_t st, int sms) {
+  TcArgs a;
+  memset(&a, 0, sizeof(a));
+  const T* d = static_cast<const T*>(dgu);
+  const T* d0 = dwg ? d : d + g.F;  // one weight wanted alone is the first half, and there is no second
+  int rc;
+  if ((rc = box_map<T>(&a.a0, d0, g.F, g.M, 2ll * g.F, 64)) || (rc = box_map<T>(&a.a1, d + g.F, g.F, g.M, 2ll * g.F, 64)) ||
+      (rc = box_map<T>(&a.b0, g.x, g.K, g.M, g.ldx, 64)))
+    return rc;
+  a.rows = g.F, a.cols = g.K, a.depth = g.M;
+  a.tiles_half = (g.F + 255) / 256, a.tiles_j = (g.K + 255) / 256;
+  a.tiles_i = dwg && dwu ? 2 * a.tiles_half : a.tiles_half;
+  a.panel = 16, a.i_fast = 0;
+  a.out0 = dwg ? dwg : dwu, a.out1 = dwu, a.ld = g.K;
+  a.wide = rows32(a.out0, g.K) && rows32(a.out1, g.K);
+  return launch_pair<T, kWeightGrad, kSilu>(a, st, sms);
+}
+
+}  // namespace gated
+
+int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::forward_tc<__half>(a, act, h, save, st, sms)
+                                : gated::forward_tc<__nv_bfloat16>(a, act, h, save, st, sms);
+}
+
+int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, cudaStream_t st, int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::input_grad_tc<__half>(a, dgu, dx, st, sms)
+                                : gated::input_grad_tc<__nv_bfloat16>(a, dgu, dx, st, sms);
+}
+
+int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, cudaStream_t st,
+                             int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::weight_grad_tc<__half>(a, dgu, dwg, dwu, st, sms)
+                                : gated::weight_grad_tc<__nv_bfloat16>(a, dgu, dwg, dwu, st, sms);
+}
+
+}  // namespace gfx

@@ -161,6 +161,12 @@ int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float*
 int launch_gated_backward(const GatedArgs& a, int dtype, int act, const void* dh, long long ldh, const float* save,
                           const GatedGrads& d, void* workspace, cudaStream_t st, int sms);
 size_t gated_backward_workspace(int M, int F);
+// its matrix products on the tensor cores -- gated_tc.cu (dgu [M, 2F]: dg, then du)
+int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms);
+int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, cudaStream_t st, int sms);
+int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, cudaStream_t st,
+                             int sms);
+int gated_tc_device_status(int clear);
 
 // loaders / helpers -- pack.cu
 int launch_int4_dequant(const void* wq, const void* ws, int scale_dtype, void* out, int out_dtype, int N, int K,

@@ -93,8 +93,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
         if t is not None and tuple(t.shape) != (N,):
             raise RuntimeError(f"{name} must have {N} elements, got {tuple(t.shape)}")
     x2 = x.reshape(-1, K)
-    if x2.shape[0] > 2 ** 31 - 1:
-        raise RuntimeError(f"at most 2^31 - 1 tokens, got {x2.shape[0]}")
+    if x2.shape[0] > 2 ** 30:
+        raise RuntimeError(f"at most 2^30 tokens, got {x2.shape[0]}")
     b_gate, b_up = (b.contiguous() if b is not None else None for b in (b_gate, b_up))
     h = _GatedLinear.apply(_rows(x2), _rows(w_gate), _rows(w_up), b_gate, b_up, ACTIVATIONS[activation])
     return h.reshape(*x.shape[:-1], N)
