@@ -83,10 +83,11 @@ SIGNATURES = {
                                                                 ctypes.c_float, _c_void_p, _c_size_t, _c_void_p]),
     "qk_norm_rope_workspace_bytes": (_c_size_t, [_c_int]),
     "gated_linear": (_c_int, [_c_void_p, _c_int64] * 3 + [_c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p,
-                                                          _c_int, _c_int, _c_int, _c_void_p]),
+                                                          _c_int, _c_int, _c_int, _c_void_p, _c_size_t, _c_void_p]),
+    "gated_linear_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "gated_linear_backward": (_c_int, [_c_void_p, _c_int64] * 4 + [_c_void_p, _c_int, _c_int] + [_c_void_p] * 5 +
                               [_c_int] * 3 + [_c_void_p, _c_size_t, _c_void_p]),
-    "gated_linear_backward_workspace_bytes": (_c_size_t, [_c_int, _c_int]),
+    "gated_linear_backward_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "w4a4_gemm_exact": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                                  _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_size_t, _c_void_p]),
 }

@@ -243,8 +243,9 @@ int gfx_device_status(int clear) {
   int v = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return -set_error(GFX_ERR_CUDA, "gfx_device_status: %s", cudaGetErrorString(e));
-  const int parts[6] = {smallm_device_status(clear), tc_device_status(clear), selftest_device_status(clear),
-                         w4a4x_device_status(clear), attn_tc_device_status(clear), gated_tc_device_status(clear)};
+  const int parts[7] = {smallm_device_status(clear), tc_device_status(clear), selftest_device_status(clear),
+                         w4a4x_device_status(clear), attn_tc_device_status(clear), gated_tc_device_status(clear),
+                         gated_few_device_status(clear)};
   for (int p : parts) {
     if (p < 0) return -set_error(GFX_ERR_CUDA, "gfx_device_status: reading a status word failed");
     if (p && !v) v = p;
@@ -833,7 +834,7 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
                  const void* b_gate, const void* b_up, int dtype, int act, void* h, float* save, int M, int K, int F,
-                 gfx_stream_t stream) {
+                 void* workspace, size_t workspace_bytes, gfx_stream_t stream) {
   const char* fn = "gated_linear";
   GatedArgs a;
   int rc = gated_common(fn, &a, x, ldx, w_gate, ldg, w_up, ldu, dtype, act, M, K, F);
@@ -847,12 +848,23 @@ int gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, co
   a.b_gate = b_gate, a.b_up = b_up;
   const int dev = current_device();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if ((rc = check_device_health(fn, dev, nullptr, 0, st))) return rc;
-  return launch_gated_forward(a, dtype, act, h, save, st, sm_count(dev));
+  const int sms = sm_count(dev);
+  const size_t need = gated_forward_workspace(M, K, F, sms);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(GFX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", fn, need,
+                     workspace ? workspace_bytes : (size_t)0);
+  if ((rc = check_device_health(fn, dev, need ? workspace : nullptr,
+                                need < kSplitKCounterBytes ? need : kSplitKCounterBytes, st)))
+    return rc;
+  return launch_gated_forward(a, dtype, act, h, save, need ? workspace : nullptr, st, sms);
 }
 
-size_t gated_linear_backward_workspace_bytes(int M, int F) {
-  return M <= 0 || F <= 0 ? 0 : gated_backward_workspace(M, F);
+size_t gated_linear_workspace_bytes(int M, int K, int F) {
+  return M <= 0 || K <= 0 || F <= 0 ? 0 : gated_forward_workspace(M, K, F, sm_count(current_device()));
+}
+
+size_t gated_linear_backward_workspace_bytes(int M, int K, int F) {
+  return M <= 0 || K <= 0 || F <= 0 ? 0 : gated_backward_workspace(M, K, F, sm_count(current_device()));
 }
 
 int gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
@@ -882,12 +894,14 @@ int gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t l
   }
   if (!dh || !save || ((dw_gate || dw_up) && !x) || (dx && (!w_gate || !w_up)))
     return set_error(GFX_ERR_INVALID, "%s: dh, save, or an operand of a gradient that is asked for is a null pointer", fn);
-  if (!workspace || workspace_bytes < gated_backward_workspace(M, F) || !aligned16(workspace))
-    return set_error(GFX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", fn,
-                     gated_backward_workspace(M, F), workspace ? workspace_bytes : (size_t)0);
+  const int sms = sm_count(dev);
+  const size_t need = gated_backward_workspace(M, K, F, sms);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return set_error(GFX_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", fn, need,
+                     workspace ? workspace_bytes : (size_t)0);
   if ((rc = check_device_health(fn, dev, nullptr, 0, st))) return rc;
   const GatedGrads d{dx, dw_gate, dw_up, db_gate, db_up};
-  return launch_gated_backward(a, dtype, act, dh, lddh, save, d, workspace, st, sm_count(dev));
+  return launch_gated_backward(a, dtype, act, dh, lddh, save, d, workspace, st, sms);
 }
 
 }  // extern "C"

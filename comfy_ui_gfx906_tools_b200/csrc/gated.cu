@@ -25,7 +25,10 @@ constexpr int kRowsPerBlock = 64;
 
 template <typename T, int kAct>
 __global__ void __launch_bounds__(256) gate_grad_kernel(const T* dh, long long ldh, const float* save, T* dgu,
-                                                        float* partial, int M, int F) {
+                                                        float* partial, int* counters, int M, int F) {
+  // the products that follow want their counters at zero
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < (int)(kGatedCounterBytes / sizeof(int)); i += 256) counters[i] = 0;
   // a warp: 128 columns (4 a lane) of every eighth row
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int f = blockIdx.y * 128 + lane * 4;
@@ -85,24 +88,41 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const float* partial, in
 
 static int row_blocks(int M) { return (M + gated::kRowsPerBlock - 1) / gated::kRowsPerBlock; }
 
-size_t gated_backward_workspace(int M, int F) {
-  return align_up((size_t)M * 2 * F * 2, 256) + (size_t)row_blocks(M) * 2 * F * sizeof(float);
+size_t gated_forward_workspace(int M, int K, int F, int sms) {
+  return M <= kGatedFewTokens ? 0 : gated_forward_tc_workspace(M, K, F, sms);
 }
 
-int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms) {
-  return launch_gated_forward_tc(a, dtype, act, h, save, st, sms);
+int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, void* workspace,
+                         cudaStream_t st, int sms) {
+  if (a.M <= kGatedFewTokens) return launch_gated_forward_few(a, dtype, act, h, save, st, sms);
+  return launch_gated_forward_tc(a, dtype, act, h, save, workspace, st, sms);
+}
+
+// The backward's workspace: counters and sums of the products, dg and du, the column sums.
+static size_t dgu_offset(const GatedArgs& a, int sms) {
+  return align_up(gated_backward_tc_workspace(a.M, a.K, a.F, sms), 256);
+}
+static size_t sums_offset(const GatedArgs& a, int sms) {
+  return dgu_offset(a, sms) + align_up((size_t)a.M * 2 * a.F * 2, 256);
+}
+
+size_t gated_backward_workspace(int M, int K, int F, int sms) {
+  GatedArgs a{};
+  a.M = M, a.K = K, a.F = F;
+  return sums_offset(a, sms) + (size_t)row_blocks(M) * 2 * F * sizeof(float);
 }
 
 template <typename T>
 static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long long ldh, const float* save,
                             const GatedGrads& d, void* workspace, cudaStream_t st, int sms) {
-  T* dgu = static_cast<T*>(workspace);
-  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up((size_t)a.M * 2 * a.F * 2, 256));
+  char* ws = static_cast<char*>(workspace);
+  T* dgu = reinterpret_cast<T*>(ws + dgu_offset(a, sms));
+  float* partial = reinterpret_cast<float*>(ws + sums_offset(a, sms));
   const int blocks = row_blocks(a.M);
   const bool bias = d.b_gate || d.b_up;
   const dim3 grid(blocks, (a.F + 127) / 128);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, st>>>((const T*)dh, ldh, save, dgu, bias ? partial : nullptr, a.M, a.F);
+    kern<<<grid, 256, 0, st>>>((const T*)dh, ldh, save, dgu, bias ? partial : nullptr, static_cast<int*>(workspace), a.M, a.F);
   };
   if (act == gated::kSilu)
     go(gated::gate_grad_kernel<T, gated::kSilu>);
@@ -117,8 +137,8 @@ static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long lo
     if ((rc = check_launch("bias_grad_kernel"))) return rc;
   }
   constexpr int kDtype = std::is_same<T, __half>::value ? GFX_DTYPE_F16 : GFX_DTYPE_BF16;
-  if (d.x && (rc = launch_gated_input_grad(a, kDtype, dgu, d.x, st, sms))) return rc;
-  if (d.w_gate || d.w_up) return launch_gated_weight_grad(a, kDtype, dgu, d.w_gate, d.w_up, st, sms);
+  if (d.x && (rc = launch_gated_input_grad(a, kDtype, dgu, d.x, workspace, st, sms))) return rc;
+  if (d.w_gate || d.w_up) return launch_gated_weight_grad(a, kDtype, dgu, d.w_gate, d.w_up, workspace, st, sms);
   return GFX_OK;
 }
 

@@ -33,6 +33,14 @@
 // loaded while the second block's accumulator is still read. A stage's barrier
 // lives in CTA 0 and counts both CTAs' bytes. Persistent: one pair per two
 // SMs; tiles are walked in panels whose reused operand stays in L2.
+//
+// Tiles that do not fill a last wave are cut along the contraction, so that
+// all pairs work on them at once (dx of 4608 x 3072 is 108 tiles for 74 pairs:
+// 74 whole ones, then 34 in two halves each). The pairs of a wave move along
+// the contraction side by side, which keeps the shared operands in L2; ranges
+// that start anywhere would not. Each epilogue warp leaves its sums of a cut
+// tile in the workspace and counts itself in; the last one of a tile adds all
+// parts in their order, so the result does not depend on who came last.
 #include <string.h>
 
 #include <type_traits>
@@ -69,6 +77,9 @@ struct TcArgs {
   int depth;            // of the contraction, per segment (K; F; M)
   int tiles_i, tiles_j; // row tiles and column tiles
   int tiles_half;       // dW: row tiles of one weight; the second's follow
+  int whole, cut, parts;// tiles taken whole, and those cut in `parts` along the contraction
+  float* partial;       // sums of cut tiles, [cut * parts][2 CTAs][blocks][8 warps][128][32]
+  int* counters;        // [cut][2][blocks][8], zero between calls
   int panel;            // tiles of the fast direction that are walked before the slow one moves
   int i_fast;
   void* out0;           // h; dx; dWg
@@ -167,6 +178,25 @@ __device__ __forceinline__ void tile_at(const TcArgs& a, int t, int& i, int& j) 
   j = a.i_fast ? s : f;
 }
 
+// What a pair does at once: a tile, or one part of a cut tile.
+struct Unit {
+  int tile, part, k0, k1;  // part -1: the whole tile
+};
+
+__device__ __forceinline__ Unit unit_at(const TcArgs& a, int u, int total) {
+  Unit w{u, -1, 0, total};
+  if (u >= a.whole) {
+    const int v = u - a.whole;
+    w.tile = a.whole + v % a.cut;
+    if (a.parts > 1) {
+      w.part = v / a.cut;
+      w.k0 = (int)((long long)total * w.part / a.parts);
+      w.k1 = (int)((long long)total * (w.part + 1) / a.parts);
+    }
+  }
+  return w;
+}
+
 template <typename T, int kRole, int kAct, int kBlocks>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_kernel(const __grid_constant__ TcArgs a) {
   constexpr int kStages = Ring<kBlocks>::kStages, kStageBytes = Ring<kBlocks>::kStageBytes;
@@ -182,10 +212,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cr = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = a.tiles_i * a.tiles_j;
-  const int segments = kRole == kInputGrad ? 2 : 1;
+  const int units = a.whole + a.cut * a.parts;
   const int steps = (a.depth + kStageK - 1) / kStageK;  // per segment
-  const int total = steps * segments;
+  const int stages = kRole == kInputGrad ? 2 * steps : steps;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -211,13 +240,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
       tma_prefetch_desc(&a.a0);
       tma_prefetch_desc(&a.b0);
       uint32_t it = 0;
-      for (int t = pair; t < tiles && ok; t += pairs) {
+      for (int u = pair; u < units && ok; u += pairs) {
+        const Unit w = unit_at(a, u, stages);
         int i, j;
-        tile_at(a, t, i, j);
+        tile_at(a, w.tile, i, j);
         const int half = kRole == kWeightGrad && i >= a.tiles_half;
         const int r0 = (half ? i - a.tiles_half : i) * (kBlocks * kBlockRows) + (int)cr * 128;
         const int c0 = kRole == kForward ? j * 128 : j * kTileCols + (int)cr * 128;
-        for (int k = 0; k < total; ++k, ++it) {
+        for (int k = w.k0; k < w.k1; ++k, ++it) {
           const int seg = k >= steps ? 1 : 0;
           const CUtensorMap* am = (kRole == kWeightGrad ? half : seg) ? &a.a1 : &a.a0;
           const CUtensorMap* bm = (kRole == kForward ? (int)cr : kRole == kInputGrad ? seg : 0) ? &a.b1 : &a.b0;
@@ -280,7 +310,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
       };
       uint32_t it = 0;
       int n = 0;
-      for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+      for (int u = pair; u < units && ok; u += pairs, ++n) {
+        const Unit w = unit_at(a, u, stages);
+        const int total = w.k1 - w.k0;
         int k = 0;
         if constexpr (kBlocks == 2) {
           // the first stages: the first block as soon as its accumulator is free, then the second
@@ -338,9 +370,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
   } else {
     const int quadrant = warp & 3, side = warp >> 2;  // 32 TMEM lanes; which half of the columns
     int n = 0;
-    for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+    for (int u = pair; u < units && ok; u += pairs, ++n) {
+      const Unit w = unit_at(a, u, stages);
       int i, j;
-      tile_at(a, t, i, j);
+      tile_at(a, w.tile, i, j);
       const int half = kRole == kWeightGrad && i >= a.tiles_half;
       const int row0 = (half ? i - a.tiles_half : i) * (kBlocks * kBlockRows) + (int)cr * 128 + quadrant * 32 + lane;
 #pragma unroll 1
@@ -366,6 +399,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(&acc_empty[acc], 0);
+        if (w.part >= 0) {
+          // this warp's values of part p of the tile: 32 groups of four per lane
+          const int place = ((w.tile - a.whole) * 2 + (int)cr) * kBlocks * 8 + b * 8 + warp;
+          const long long part_size = (long long)a.cut * 2 * kBlocks * 8 * 4096;
+          float* region = a.partial + (long long)place * 4096 + lane * 4;
+          float* mine = region + w.part * part_size;
+#pragma unroll
+          for (int g = 0; g < 32; ++g) {
+            const uint32_t* x = &v[g / 8][g % 8 * 4];
+            st_global_v4(mine + g * 128, x[0], x[1], x[2], x[3]);
+          }
+          __threadfence();
+          __syncwarp();
+          int before = 0;
+          if (lane == 0) before = atomicAdd(&a.counters[place], 1);
+          if (__shfl_sync(0xFFFFFFFFu, before, 0) != a.parts - 1) continue;
+          __threadfence();
+          if (lane == 0) a.counters[place] = 0;
+          // The parts come through this warp's 16 KB of the stages' memory, which is free: a pair's cut tile is the
+          // last thing it does, and its loads and MMAs (the second block's too) are done. Two parts: the other one is
+          // added to the registers (a sum of two has no order). More: all of them, from the first on.
+          if (kBlocks == 2 && b == 0 && !mbar_wait(&acc_full[1], n & 1, kDevErrEpilogueBarrierTimeout)) {
+            ok = false;
+            break;
+          }
+          const bool two = a.parts == 2;
+          uint8_t* buf = base + warp * 16384 + lane * 16;
+          if (!two) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[q][e] = 0u;
+          }
+#pragma unroll 1
+          for (int p = two ? 1 - w.part : 0; p < (two ? 2 - w.part : a.parts); ++p) {
+            const float* theirs = region + p * part_size;
+#pragma unroll
+            for (int g = 0; g < 32; ++g) cp_async_16(buf + g * 512, theirs + g * 128, 16);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+            for (int g = 0; g < 32; ++g) {
+              const uint4 x = lds128(smem_u32(buf) + g * 512);
+              uint32_t* to = &v[g / 8][g % 8 * 4];
+              to[0] = __float_as_uint(__uint_as_float(to[0]) + __uint_as_float(x.x));
+              to[1] = __float_as_uint(__uint_as_float(to[1]) + __uint_as_float(x.y));
+              to[2] = __float_as_uint(__uint_as_float(to[2]) + __uint_as_float(x.z));
+              to[3] = __float_as_uint(__uint_as_float(to[3]) + __uint_as_float(x.w));
+            }
+          }
+        }
         if constexpr (kRole == kForward) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -434,27 +517,58 @@ static int launch_pair_blocks(TcArgs& a, cudaStream_t st, int sms) {
     }
     pairs_at_once[dev] = n < sms / 2 ? n : sms / 2;
   }
-  const int tiles = a.tiles_i * a.tiles_j;
-  cfg.gridDim = dim3(2 * (tiles < pairs_at_once[dev] ? tiles : pairs_at_once[dev]));
+  // a pair takes at most one part of a cut tile (it uses the stages' memory to join them)
+  if (a.cut * a.parts > pairs_at_once[dev]) a.parts = 1;
+  const int units = a.whole + a.cut * a.parts;
+  cfg.gridDim = dim3(2 * (units < pairs_at_once[dev] ? units : pairs_at_once[dev]));
   a.status_host = host_status_word(dev);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(GFX_ERR_CUDA, "gated pair_kernel launch: %s", cudaGetErrorString(e));
   return check_launch("gated pair_kernel");
 }
 
-// `rows` and `halves` of them (dW: both weights') in row blocks: two a tile, unless one leaves the GPU less idle.
-// A wave of two-block tiles takes twice the MMAs of a wave of one-block tiles at 1.35 times their rate.
-template <typename T, int kRole, int kAct>
-static int launch_pair(TcArgs& a, int halves, cudaStream_t st, int sms) {
-  const long long one = (a.rows + kBlockRows - 1) / kBlockRows, two = (a.rows + 2 * kBlockRows - 1) / (2 * kBlockRows);
-  const long long pairs = sms / 2;
-  const long long waves1 = (one * halves * a.tiles_j + pairs - 1) / pairs;
-  const long long waves2 = (two * halves * a.tiles_j + pairs - 1) / pairs;
-  const bool second = waves2 * 200 < waves1 * 135;
-  a.tiles_half = (int)(second ? two : one);
-  a.tiles_i = a.tiles_half * halves;
-  return second ? launch_pair_blocks<T, kRole, kAct, 2>(a, st, sms) : launch_pair_blocks<T, kRole, kAct, 1>(a, st, sms);
+struct Plan {
+  int blocks, tiles_half, whole, cut, parts;
+  size_t partial_bytes() const { return parts > 1 ? (size_t)cut * parts * 2 * blocks * 8 * 4096 * sizeof(float) : 0; }
+};
+
+// Row blocks a tile, and the cut of the last wave, by the cycles that they take: a stage of 64 along the contraction
+// is 780 cycles with one row block and 1150 with two (measured: 66% and 89% of the tensor cores' rate); joining the
+// parts of a tile takes some 6000 a block for the exchange and 3000 for each part that is read. `rows` in `halves` (dW: both weights'), `stages` along the contraction.
+static Plan make_plan(long long rows, int halves, int tiles_j, int stages, bool may_cut, int sms) {
+  const int pairs = sms / 2;
+  Plan best{};
+  double least = 0.0;
+  for (int blocks = 1; blocks <= 2; ++blocks) {
+    const int half = (int)((rows + blocks * kBlockRows - 1) / (blocks * kBlockRows));
+    const int tiles = half * halves * tiles_j, rest = tiles % pairs;
+    const double wave = (double)stages * (blocks == 1 ? 780 : 1150);
+    for (int parts = 1; parts <= 8; ++parts) {
+      if (parts > 1 && (!may_cut || rest == 0 || rest * parts > pairs || stages / parts < 4)) break;
+      const double t = tiles / pairs * wave + (rest ? wave / parts : 0.0) + (parts > 1 ? (6000.0 + 3000.0 * (parts == 2 ? 1 : parts)) * blocks : 0.0);
+      if (best.blocks == 0 || t < least) {
+        least = t;
+        best = Plan{blocks, half, tiles - rest, rest, parts};
+      }
+    }
+  }
+  return best;
 }
+
+// workspace: the counters' region and then plan.partial_bytes(); null: no tile is cut.
+template <typename T, int kRole, int kAct>
+static int launch_pair(TcArgs& a, int halves, int stages, void* workspace, cudaStream_t st, int sms) {
+  const Plan p = make_plan(a.rows, halves, a.tiles_j, stages, workspace != nullptr, sms);
+  a.tiles_half = p.tiles_half;
+  a.tiles_i = p.tiles_half * halves;
+  a.whole = p.whole, a.cut = p.cut, a.parts = p.parts;
+  a.counters = static_cast<int*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSplitKCounterBytes);
+  return p.blocks == 2 ? launch_pair_blocks<T, kRole, kAct, 2>(a, st, sms)
+                       : launch_pair_blocks<T, kRole, kAct, 1>(a, st, sms);
+}
+
+static int stages_of(int depth) { return (depth + kStageK - 1) / kStageK; }
 
 template <typename T>
 constexpr CUtensorMapDataType map_type() {
@@ -471,7 +585,8 @@ static int box_map(CUtensorMap* m, const void* p, long long inner, long long out
 static bool rows32(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0 && ld % 16 == 0; }
 
 template <typename T>
-static int forward_tc(const GatedArgs& g, int act, void* h, float* save, cudaStream_t st, int sms) {
+static int forward_tc(const GatedArgs& g, int act, void* h, float* save, void* workspace, cudaStream_t st,
+                      int sms) {
   TcArgs a;
   memset(&a, 0, sizeof(a));
   int rc;
@@ -483,14 +598,14 @@ static int forward_tc(const GatedArgs& g, int act, void* h, float* save, cudaStr
   a.panel = 16, a.i_fast = 1;
   a.out0 = h, a.ld = g.F, a.bias0 = g.b_gate, a.bias1 = g.b_up, a.save = save;
   a.wide = rows32(h, g.F) && (reinterpret_cast<uintptr_t>(save) & 31) == 0;
-  if (act == kSilu) return launch_pair<T, kForward, kSilu>(a, 1, st, sms);
-  if (act == kGelu) return launch_pair<T, kForward, kGelu>(a, 1, st, sms);
-  return launch_pair<T, kForward, kGeluTanh>(a, 1, st, sms);
+  if (act == kSilu) return launch_pair<T, kForward, kSilu>(a, 1, stages_of(g.K), workspace, st, sms);
+  if (act == kGelu) return launch_pair<T, kForward, kGelu>(a, 1, stages_of(g.K), workspace, st, sms);
+  return launch_pair<T, kForward, kGeluTanh>(a, 1, stages_of(g.K), workspace, st, sms);
 }
 
 // dx [M, K] from dgu [M, 2F]
 template <typename T>
-static int input_grad_tc(const GatedArgs& g, const void* dgu, void* dx, cudaStream_t st, int sms) {
+static int input_grad_tc(const GatedArgs& g, const void* dgu, void* dx, void* workspace, cudaStream_t st, int sms) {
   TcArgs a;
   memset(&a, 0, sizeof(a));
   const T* d = static_cast<const T*>(dgu);
@@ -503,12 +618,13 @@ static int input_grad_tc(const GatedArgs& g, const void* dgu, void* dx, cudaStre
   a.panel = 16, a.i_fast = 1;
   a.out0 = dx, a.ld = g.K;
   a.wide = rows32(dx, g.K);
-  return launch_pair<T, kInputGrad, kSilu>(a, 1, st, sms);
+  return launch_pair<T, kInputGrad, kSilu>(a, 1, 2 * stages_of(g.F), workspace, st, sms);
 }
 
 // dWg, dWu [F, K]: both, or one of them
 template <typename T>
-static int weight_grad_tc(const GatedArgs& g, const void* dgu, void* dwg, void* dwu, cudaStream_t st, int sms) {
+static int weight_grad_tc(const GatedArgs& g, const void* dgu, void* dwg, void* dwu, void* workspace,
+                          cudaStream_t st, int sms) {
   TcArgs a;
   memset(&a, 0, sizeof(a));
   const T* d = static_cast<const T*>(dgu);
@@ -522,25 +638,43 @@ static int weight_grad_tc(const GatedArgs& g, const void* dgu, void* dwg, void* 
   a.panel = 16, a.i_fast = 0;
   a.out0 = dwg ? dwg : dwu, a.out1 = dwu, a.ld = g.K;
   a.wide = rows32(a.out0, g.K) && rows32(a.out1, g.K);
-  return launch_pair<T, kWeightGrad, kSilu>(a, dwg && dwu ? 2 : 1, st, sms);
+  return launch_pair<T, kWeightGrad, kSilu>(a, dwg && dwu ? 2 : 1, stages_of(g.M), workspace, st, sms);
 }
 
 }  // namespace gated
 
-int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms) {
-  return dtype == GFX_DTYPE_F16 ? gated::forward_tc<__half>(a, act, h, save, st, sms)
-                                : gated::forward_tc<__nv_bfloat16>(a, act, h, save, st, sms);
+size_t gated_forward_tc_workspace(int M, int K, int F, int sms) {
+  const size_t n = gated::make_plan(M, 1, (F + 127) / 128, gated::stages_of(K), true, sms).partial_bytes();
+  return n ? kSplitKCounterBytes + n : 0;
 }
 
-int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, cudaStream_t st, int sms) {
-  return dtype == GFX_DTYPE_F16 ? gated::input_grad_tc<__half>(a, dgu, dx, st, sms)
-                                : gated::input_grad_tc<__nv_bfloat16>(a, dgu, dx, st, sms);
+size_t gated_backward_tc_workspace(int M, int K, int F, int sms) {
+  using namespace gated;
+  const int tiles_j = (K + 255) / 256;
+  size_t n = make_plan(M, 1, tiles_j, 2 * stages_of(F), true, sms).partial_bytes();
+  for (int halves = 1; halves <= 2; ++halves) {
+    const size_t w = make_plan(F, halves, tiles_j, stages_of(M), true, sms).partial_bytes();
+    n = w > n ? w : n;
+  }
+  return kSplitKCounterBytes + n;
 }
 
-int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, cudaStream_t st,
-                             int sms) {
-  return dtype == GFX_DTYPE_F16 ? gated::weight_grad_tc<__half>(a, dgu, dwg, dwu, st, sms)
-                                : gated::weight_grad_tc<__nv_bfloat16>(a, dgu, dwg, dwu, st, sms);
+int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, void* workspace,
+                            cudaStream_t st, int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::forward_tc<__half>(a, act, h, save, workspace, st, sms)
+                                : gated::forward_tc<__nv_bfloat16>(a, act, h, save, workspace, st, sms);
+}
+
+int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, void* workspace, cudaStream_t st,
+                            int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::input_grad_tc<__half>(a, dgu, dx, workspace, st, sms)
+                                : gated::input_grad_tc<__nv_bfloat16>(a, dgu, dx, workspace, st, sms);
+}
+
+int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, void* workspace,
+                             cudaStream_t st, int sms) {
+  return dtype == GFX_DTYPE_F16 ? gated::weight_grad_tc<__half>(a, dgu, dwg, dwu, workspace, st, sms)
+                                : gated::weight_grad_tc<__nv_bfloat16>(a, dgu, dwg, dwu, workspace, st, sms);
 }
 
 }  // namespace gfx

@@ -156,17 +156,30 @@ struct GatedArgs {
 struct GatedGrads {  // null: not wanted
   void *x, *w_gate, *w_up, *b_gate, *b_up;
 };
-// save: float32 [2][M][F] (g, then u), or null
-int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms);
+// save: float32 [2][M][F] (g, then u), or null. The forward's workspace has its counters (zero before its first use,
+// left at zero) in front; the backward's may hold anything.
+size_t gated_forward_workspace(int M, int K, int F, int sms);
+int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, void* workspace,
+                         cudaStream_t st, int sms);
+size_t gated_backward_workspace(int M, int K, int F, int sms);
 int launch_gated_backward(const GatedArgs& a, int dtype, int act, const void* dh, long long ldh, const float* save,
                           const GatedGrads& d, void* workspace, cudaStream_t st, int sms);
-size_t gated_backward_workspace(int M, int F);
-// its matrix products on the tensor cores -- gated_tc.cu (dgu [M, 2F]: dg, then du)
-int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms);
-int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, cudaStream_t st, int sms);
-int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, cudaStream_t st,
-                             int sms);
+// its matrix products on the tensor cores -- gated_tc.cu (dgu [M, 2F]: dg, then du). workspace: kSplitKCounterBytes of
+// counters (the first kGatedCounterBytes are used: zero, and left at zero), then the sums of cut tiles.
+constexpr size_t kGatedCounterBytes = 16 * 1024;
+size_t gated_forward_tc_workspace(int M, int K, int F, int sms);   // 0: none needed
+size_t gated_backward_tc_workspace(int M, int K, int F, int sms);
+int launch_gated_forward_tc(const GatedArgs& a, int dtype, int act, void* h, float* save, void* workspace,
+                            cudaStream_t st, int sms);
+int launch_gated_input_grad(const GatedArgs& a, int dtype, const void* dgu, void* dx, void* workspace, cudaStream_t st,
+                            int sms);
+int launch_gated_weight_grad(const GatedArgs& a, int dtype, const void* dgu, void* dwg, void* dwu, void* workspace,
+                             cudaStream_t st, int sms);
 int gated_tc_device_status(int clear);
+// its form for few tokens -- gated_few.cu
+constexpr int kGatedFewTokens = 128;
+int launch_gated_forward_few(const GatedArgs& a, int dtype, int act, void* h, float* save, cudaStream_t st, int sms);
+int gated_few_device_status(int clear);
 
 // loaders / helpers -- pack.cu
 int launch_int4_dequant(const void* wq, const void* ws, int scale_dtype, void* out, int out_dtype, int N, int K,

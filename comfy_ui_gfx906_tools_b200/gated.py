@@ -39,9 +39,11 @@ class _GatedLinear(torch.autograd.Function):
         if any(ctx.needs_input_grad[:5]):
             save = torch.empty(2, M, N, dtype=torch.float32, device=x.device)
         with torch.cuda.device(x.device):
-            _lib.call("gated_linear", x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(),
-                      w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._dtype_code(x.dtype), act, h.data_ptr(),
-                      _ptr(save), M, K, N, ops._stream(x.device))
+            stream = ops._stream(x.device)
+            ws = ops._workspace(x.device, stream, _lib.load().gated_linear_workspace_bytes(M, K, N))
+            ops._call_gemm("gated_linear", x.device, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0),
+                           w_up.data_ptr(), w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._dtype_code(x.dtype), act,
+                           h.data_ptr(), _ptr(save), M, K, N, _ptr(ws), ws.numel() if ws is not None else 0, stream)
         ctx.act = act
         ctx.save_for_backward(x, w_gate, w_up, save)
         return h
@@ -56,12 +58,12 @@ class _GatedLinear(torch.autograd.Function):
         grads = [torch.empty(s, dtype=x.dtype, device=x.device) if need else None
                  for s, need in zip(shapes, ctx.needs_input_grad)]
         with torch.cuda.device(x.device):
-            ws = torch.empty(_lib.load().gated_linear_backward_workspace_bytes(M, N), dtype=torch.uint8,
+            ws = torch.empty(_lib.load().gated_linear_backward_workspace_bytes(M, K, N), dtype=torch.uint8,
                              device=x.device)
-            _lib.call("gated_linear_backward", dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0),
-                      w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), save.data_ptr(),
-                      ops._dtype_code(x.dtype), ctx.act, *map(_ptr, grads), M, K, N, ws.data_ptr(), ws.numel(),
-                      ops._stream(x.device))
+            ops._call_gemm("gated_linear_backward", x.device, dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0),
+                           w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), save.data_ptr(),
+                           ops._dtype_code(x.dtype), ctx.act, *map(_ptr, grads), M, K, N, ws.data_ptr(), ws.numel(),
+                           ops._stream(x.device))
         return (*grads, None)
 
 

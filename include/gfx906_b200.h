@@ -395,23 +395,28 @@ size_t qk_norm_rope_workspace_bytes(int D);
  *   act: 0 silu, 1 gelu (erf), 2 gelu with the tanh approximation.
  *   save: float32 [2][M][F] that receives g and u for the backward, or NULL.
  * Products accumulate in float32; h is rounded once.
+ * workspace: gated_linear_workspace_bytes(M, K, F) bytes (may be 0), 16-byte
+ * aligned; its counters, the first 256 KB, must hold zeros before its first
+ * use, and every call leaves them at zero (one workspace serves every
+ * operator with this contract, on one stream).
  */
 int gated_linear(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu,
                  const void* b_gate, const void* b_up, int dtype, int act, void* h, float* save, int M, int K, int F,
-                 gfx_stream_t stream);
+                 void* workspace, size_t workspace_bytes, gfx_stream_t stream);
+size_t gated_linear_workspace_bytes(int M, int K, int F);
 /*
  * Its gradients from dh [M, F] (row stride lddh, a multiple of 8) and the
  * forward's save:
  *   dx [M, K], dw_gate / dw_up [F, K], db_gate / db_up [F], dense, of dtype;
  *   each may be NULL (not computed). x is read only for the weights' gradients.
- * workspace: gated_linear_backward_workspace_bytes(M, F) bytes, 16-byte
+ * workspace: gated_linear_backward_workspace_bytes(M, K, F) bytes, 16-byte
  * aligned, any contents.
  */
 int gated_linear_backward(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
                           const void* w_up, int64_t ldu, const float* save, int dtype, int act, void* dx,
                           void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int K, int F, void* workspace,
                           size_t workspace_bytes, gfx_stream_t stream);
-size_t gated_linear_backward_workspace_bytes(int M, int F);
+size_t gated_linear_backward_workspace_bytes(int M, int K, int F);
 
 #ifdef __cplusplus
 }

@@ -83,7 +83,7 @@ def test_rope_backward_checks(built_lib):
 def _gated(lib, back=False, x=16, wg=16, wu=16, h=16, save=16, bg=None, dt=2, act=0, M=3, K=64, F=72, ldx=64, ldg=64,
            ldu=64, lddh=72, ws=16, wsb=1 << 20, dx=16, dw=16):
     if not back:
-        return lib.gated_linear(x, ldx, wg, ldg, wu, ldu, bg, None, dt, act, h, save, M, K, F, None)
+        return lib.gated_linear(x, ldx, wg, ldg, wu, ldu, bg, None, dt, act, h, save, M, K, F, ws, wsb, None)
     return lib.gated_linear_backward(h, lddh, x, ldx, wg, ldg, wu, ldu, save, dt, act, dx, dw, None, bg, None, M, K, F,
                                      ws, wsb, None)
 
@@ -109,6 +109,11 @@ def test_gated_backward_checks(built_lib):
     assert _gated(built_lib, True, ws=None) == WORKSPACE
     assert _gated(built_lib, True, ws=24) == WORKSPACE
     assert _gated(built_lib, True, wsb=100) == WORKSPACE and "workspace of" in _lib.last_error()
+    many = dict(M=700, K=6400, ldx=6400, ldg=6400, ldu=6400)  # few tiles, a long contraction: cut and joined
+    assert built_lib.gated_linear_workspace_bytes(700, 6400, 72) > 1 << 18
+    assert _gated(built_lib, False, ws=None, **many) == WORKSPACE and "workspace of" in _lib.last_error()
+    assert _gated(built_lib, False, wsb=1000, **many) == WORKSPACE
     assert _gated(built_lib, False, M=0, x=None, h=None) == _lib.GFX_OK
     assert _gated(built_lib, True, M=0, dx=None, dw=None, x=None) == _lib.GFX_OK
-    assert built_lib.gated_linear_backward_workspace_bytes(0, 8) == 0
+    assert built_lib.gated_linear_backward_workspace_bytes(0, 8, 8) == 0
+    assert built_lib.gated_linear_workspace_bytes(4, 0, 8) == 0
