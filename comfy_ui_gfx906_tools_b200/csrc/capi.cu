@@ -694,6 +694,9 @@ static int rope_common(const char* fn, RopeArgs* a, int dtype, const void* posit
     return set_error(GFX_ERR_INVALID, "%s: positions are float32 (0), int32 (1) or int64 (2), got %d", fn, pos_dtype);
   if (B < 0 || Hq < 0 || Hk < 0 || L < 0)
     return set_error(GFX_ERR_INVALID, "%s: expected B, Hq, Hk, L >= 0; got B=%d Hq=%d Hk=%d L=%d", fn, B, Hq, Hk, L);
+  if ((long long)B * L > (1 << 30) || Hq > (1 << 20) || Hk > (1 << 20))
+    return set_error(GFX_ERR_UNSUPPORTED, "%s: at most 2^30 tokens and 2^20 heads, got B=%d L=%d Hq=%d Hk=%d", fn, B, L,
+                     Hq, Hk);
   if (D <= 0 || D % 8 != 0 || D > kRopeMaxDim)
     return set_error(GFX_ERR_UNSUPPORTED, "%s: D must be a multiple of 8 up to %d, got %d", fn, kRopeMaxDim, D);
   if (!axes_dims || n_axes < 1 || n_axes > kRopeMaxAxes)
@@ -722,7 +725,7 @@ static int rope_common(const char* fn, RopeArgs* a, int dtype, const void* posit
   rope_frequencies(a, axes_dims, n_axes, theta);
   a->heads[0] = Hq, a->heads[1] = Hk;
   a->B = B, a->L = L, a->D = D;
-  a->scale_dtype = scale_dtype, a->pos_dtype = pos_dtype, a->eps = eps;
+  a->scale_dtype = scale_dtype, a->pos_dtype = pos_dtype, a->eps = eps, a->inv_dim = 1.0f / (float)D;
   a->pos = positions;
   for (int i = 0; i < 3; ++i) a->pos_stride[i] = pos_strides[i];
   a->t[0].scale = q_scale, a->t[1].scale = k_scale;

@@ -168,6 +168,12 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_cluster_v4(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
+}
+
 // Arrive with release at cluster scope on the barrier at the same offset in
 // CTA `rank`: this thread's earlier stores, distributed shared memory
 // included, are visible to a cluster-scope acquire of the completed phase.

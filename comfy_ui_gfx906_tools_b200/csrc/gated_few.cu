@@ -2,9 +2,10 @@
 // read once, whatever M is, so their bytes are what bounds it.
 //
 // The weights stand on the tensor cores' M side: a tile is 128 features, its
-// gate rows and its up rows are two accumulators D[f, m] of kN columns, kN the
-// smallest of 16, 32, 64, 128 that holds the tokens, and an MMA takes time in
-// proportion to kN. A feature's gate and up values meet in one TMEM lane, and
+// gate rows and its up rows are two accumulators D[f, m] of as many columns as
+// there are tokens (in sixteens), and an MMA takes time in proportion to them.
+// kN, the smallest of 16, 32, 64, 128 that holds them, is the accumulators'
+// place in TMEM and the room for the tokens in a stage. A feature's gate and up values meet in one TMEM lane, and
 // a warp stores 32 consecutive features of a token at once.
 //
 // With 74 tiles or more one SM takes a tile whole: that many SMs ask for more
@@ -16,7 +17,7 @@
 // through global memory by whichever CTA came last took 9 us for one token and
 // 70 for 77, against a floor of 7 to 23.)
 //
-// Warp 4 loads (TMA; gate and up tiles of 16 KB and the tokens' kN x 64 per
+// Warp 4 loads (TMA; gate and up tiles of 16 KB and the tokens per
 // stage), warp 5 issues tcgen05.mma, warps 0-3 own the 128 lanes.
 #include <string.h>
 
@@ -46,6 +47,7 @@ struct FewRing {
 struct FewArgs {
   CUtensorMap wg, wu, x;
   int M, F, steps, tiles;  // steps: K stages of a tile
+  int columns;             // tokens in sixteens: the MMA's N and the rows of x per stage
   const void* bg;
   const void* bu;
   void* h;
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(drain + 1);
   static_assert((2 * kStages + 5) * 8 + 4 <= 256, "barrier area");
-  static_assert((kN + 8) * 1024 <= kStages * kStageBytes, "the join's memory");
+  static_assert((kN + 32) * 1024 <= kStages * kStageBytes, "the join's memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int parts = (int)cluster_nctarank(), part = (int)cluster_ctarank();
   const int k0 = a.steps * part / parts, k1 = a.steps * (part + 1) / parts;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
             break;
           }
           uint8_t* st = base + s * kStageBytes;
-          mbar_arrive_expect_tx(&full[s], kStageBytes);
+          mbar_arrive_expect_tx(&full[s], 2 * kFewWeightBytes + a.columns * kFewK * 2);
           tma_load_2d(st, &a.wg, &full[s], k * kFewK, t * kFewTile);
           tma_load_2d(st + kFewWeightBytes, &a.wu, &full[s], k * kFewK, t * kFewTile);
           tma_load_2d(st + 2 * kFewWeightBytes, &a.x, &full[s], k * kFewK, 0);
@@ -138,8 +140,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
     __syncwarp();
   } else if (warp == 5) {
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    constexpr uint32_t kId = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kN >> 3) << 17) |
-                             ((uint32_t)(kFewTile >> 4) << 24);
+    const uint32_t id = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(a.columns >> 3) << 17) |
+                        ((uint32_t)(kFewTile >> 4) << 24);
     uint32_t it = 0;
     int n = 0;
     for (int t = first; t < a.tiles && ok; t += stride, ++n) {
@@ -163,8 +165,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
 #pragma unroll
           for (int q = 0; q < kFewK / 16; ++q) {
             const uint32_t more = k != k0 || q != 0;
-            tc::umma_f16<1>(tmem + acc * 2 * kN, dg + 2 * q, dx + 2 * q, kId, more);
-            tc::umma_f16<1>(tmem + acc * 2 * kN + kN, du + 2 * q, dx + 2 * q, kId, more);
+            tc::umma_f16<1>(tmem + acc * 2 * kN, dg + 2 * q, dx + 2 * q, id, more);
+            tc::umma_f16<1>(tmem + acc * 2 * kN + kN, du + 2 * q, dx + 2 * q, id, more);
           }
           tc::umma_commit<1>(&empty[s]);
           if (k == k1 - 1) tc::umma_commit<1>(&acc_full[acc]);
@@ -206,44 +208,46 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
 
   if (parts > 1) {
     // one tile a cluster; owner o finishes tokens [o share, (o + 1) share)
-    const int share = (a.M + parts - 1) / parts;
+    const int share = (a.M + 4 * parts - 1) / (4 * parts) * 4;
     cluster_sync_all();  // every CTA's loads and MMAs are done: the stages' memory is free
     if (warp < 4) {
       pdl_wait();
       if (!mbar_wait(&acc_full[0], 0, kDevErrEpilogueBarrierTimeout)) ok = false;
       tc::tc_fence_after();
       const uint32_t d = tmem + ((uint32_t)(warp * 32) << 16);
-      const uint32_t spot = smem_u32(base) + (uint32_t)(warp * 32 + lane) * 4;
-      for (int c = 0; c < a.M; c += 16) {
-        uint32_t g[16], u[16];
-        tc::tmem_ld16_nowait(d + c, g);
-        tc::tmem_ld16_nowait(d + kN + c, u);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          asm volatile("" : "+r"(g[e]), "+r"(u[e]));
-          const int m = c + e;
-          if (m < a.M) {
-            // [part][token of the owner][gate, up][128 features]
-            const uint32_t to = mapa_shared(spot + (uint32_t)((part * share + m % share) * 1024), m / share);
-            st_shared_cluster_f32(to, __uint_as_float(g[e]));
-            st_shared_cluster_f32(to + 512, __uint_as_float(u[e]));
-          }
+      // [part][four tokens of the owner][gate, up][128 features][4]: a warp stores 512 bytes in a row
+      const uint32_t spot = smem_u32(base) + (uint32_t)(part * share * 1024 + (warp * 32 + lane) * 16);
+      for (int o = 0; o * share < a.M; ++o) {
+        const uint32_t to = mapa_shared(spot, o);
+        for (int c = 0; c < share && o * share + c < a.M; c += 4) {
+          uint32_t g[4], u[4];
+          tc::tmem_ld4_nowait(d + o * share + c, g);
+          tc::tmem_ld4_nowait(d + kN + o * share + c, u);
+          tc::tmem_wait_ld();
+          asm volatile("" : "+r"(g[0]), "+r"(g[1]), "+r"(g[2]), "+r"(g[3]));
+          asm volatile("" : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]));
+          st_shared_cluster_v4(to + c * 1024, g);
+          st_shared_cluster_v4(to + c * 1024 + 2048, u);
         }
       }
       tc::tc_fence_before();
     }
     cluster_sync_all();
     const int mine = min(share, a.M - part * share);
-    const float* sums = reinterpret_cast<const float*>(base);
-    for (int i = threadIdx.x; ok && i < mine * kFewTile; i += kFewThreads) {
-      const int m = i / kFewTile, c = i % kFewTile, f = first * kFewTile + c;
-      float g = 0.0f, u = 0.0f;
+    for (int i = threadIdx.x; ok && i < (mine + 3) / 4 * kFewTile; i += kFewThreads) {
+      const int m = i / kFewTile * 4, c = i % kFewTile, f = first * kFewTile + c;
+      float g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int p = 0; p < parts; ++p) {
-        g += sums[(p * share + m) * 256 + c];
-        u += sums[(p * share + m) * 256 + 128 + c];
+        const uint32_t at = smem_u32(base) + (uint32_t)((p * share + m) * 1024 + c * 16);
+        const uint4 x = lds128(at), y = lds128(at + 2048);
+        g[0] += __uint_as_float(x.x), g[1] += __uint_as_float(x.y);
+        g[2] += __uint_as_float(x.z), g[3] += __uint_as_float(x.w);
+        u[0] += __uint_as_float(y.x), u[1] += __uint_as_float(y.y);
+        u[2] += __uint_as_float(y.z), u[3] += __uint_as_float(y.w);
       }
-      if (f < a.F) finish<T, kAct>(a, part * share + m, f, g, u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (f < a.F && m + e < mine) finish<T, kAct>(a, part * share + m + e, f, g[e], u[e]);
     }
   }
   if (!ok) mirror_device_error(a.status_host);
@@ -292,8 +296,6 @@ static int launch_few_n(FewArgs& a, int parts, cudaStream_t st, int sms) {
   return launch_few<T, kAct, 128>(a, parts, st, sms);
 }
 
-static int few_box_rows(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
-
 // CTAs a tile: as many as leave every SM at most one, at least four stages each.
 static int few_parts(int tiles, int steps, int sms) {
   int parts = sms / tiles;
@@ -307,12 +309,13 @@ static int few_t(const GatedArgs& g, int act, void* h, float* save, cudaStream_t
   memset(&a, 0, sizeof(a));
   constexpr CUtensorMapDataType kType =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  a.columns = (g.M + 15) / 16 * 16;
   int rc;
   if ((rc = make_tmap_2d(&a.wg, kType, g.w_gate, g.K, g.F, (uint64_t)g.ldg * 2, kFewK, kFewTile,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
       (rc = make_tmap_2d(&a.wu, kType, g.w_up, g.K, g.F, (uint64_t)g.ldu * 2, kFewK, kFewTile,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
-      (rc = make_tmap_2d(&a.x, kType, g.x, g.K, g.M, (uint64_t)g.ldx * 2, kFewK, few_box_rows(g.M),
+      (rc = make_tmap_2d(&a.x, kType, g.x, g.K, g.M, (uint64_t)g.ldx * 2, kFewK, a.columns,
                          CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
   a.M = g.M, a.F = g.F, a.steps = (g.K + kFewK - 1) / kFewK;

@@ -131,12 +131,14 @@ struct RopeTensor {
 struct RopeArgs {
   RopeTensor t[2];  // q, k
   int heads[2];
-  int B, L, D;
+  int B, L, D, axes;
   int pairs;        // rotated pairs
   int scale_dtype, pos_dtype;
   int vec;          // every row 16-byte aligned
-  int parts, steps_per_part;  // a token's heads in steps of 32 / lanes per row
-  float eps;
+  int steps_per_part;  // of a token's heads, 32 / lanes per row a step
+  unsigned tokens;     // B L
+  int group;           // tokens a block holds at once
+  float eps, inv_dim;
   const void* pos;
   long long pos_stride[3];  // batch, token, axis
   float* partial;           // backward: [kRopeMaxBlocks][2][D], or null

@@ -17,10 +17,14 @@
 // grow with the position (in float32 it is 1e-4 rad at position 2000, far
 // above a float32 result's rounding). Statistics and sums are float32.
 //
-// Memory-bound. A warp owns one token of a part of its heads, so a lane
-// computes the sines of its own four pairs once and reuses them for every head;
-// G = 8, 16 or 32 lanes hold a row, eight elements each (two runs of four where
-// the pairs are split halves), and a warp's rows are 32 / G heads at a time.
+// Memory-bound, but the sines cost more than the rows they turn if every warp
+// computes its own: a block of eight warps first fills a table for its 8 tokens
+// (fewer where the sequence is short), each angle once, and a warp then walks
+// the heads of one token. G = 8, 16 or 32 lanes hold a row, eight elements each
+// (two runs of four where the pairs are split halves), a warp 32 / G heads a
+// step. The rows of four steps (two in the backward, which reads two arrays)
+// are loaded before the first is used. Arithmetic is on pairs of floats, one
+// instruction for two.
 #include <math.h>
 #include <string.h>
 
@@ -32,66 +36,144 @@ namespace rotary {
 
 constexpr int kWarps = 8;
 
-// The eight elements of a lane: elements e0 .. e0 + 3 and e1 .. e1 + 3.
+// The eight elements of a lane as they lie in memory: four at p and four at p + gap.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int e0, int e1, bool vec, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    if (vec) {
-      const float4 a = *reinterpret_cast<const float4*>(row + e0), b = *reinterpret_cast<const float4*>(row + e1);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-      return;
+struct Raw {
+  uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T, bool kVec>
+__device__ __forceinline__ Raw<T> load8(const T* p, int gap) {
+  Raw<T> r;
+  if constexpr (kVec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
+      *reinterpret_cast<uint4*>(r.w + 4) = *reinterpret_cast<const uint4*>(p + gap);
+    } else if (gap == 4) {  // one run of eight
+      *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
+    } else {
+      *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p);
+      *reinterpret_cast<uint2*>(r.w + 2) = *reinterpret_cast<const uint2*>(p + gap);
     }
   } else {
-    if (vec) {
-      uint2 w[2];
-      if (e1 == e0 + 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(row + e0);
-        w[0] = make_uint2(q.x, q.y), w[1] = make_uint2(q.z, q.w);
-      } else {
-        w[0] = *reinterpret_cast<const uint2*>(row + e0);
-        w[1] = *reinterpret_cast<const uint2*>(row + e1);
-      }
-      const T* h = reinterpret_cast<const T*>(w);
+    T* h = reinterpret_cast<T*>(r.w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = to_f32<T>(h[j]);
-      return;
-    }
+    for (int j = 0; j < 4; ++j) h[j] = p[j], h[4 + j] = p[gap + j];
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = to_f32<T>(row[e0 + j]), f[4 + j] = to_f32<T>(row[e1 + j]);
+  return r;
 }
 
+// r, or zeros
 template <typename T>
-__device__ __forceinline__ void store8(T* row, int e0, int e1, bool vec, const float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    if (vec) {
-      *reinterpret_cast<float4*>(row + e0) = make_float4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<float4*>(row + e1) = make_float4(f[4], f[5], f[6], f[7]);
-      return;
+__device__ __forceinline__ Raw<T> masked(Raw<T> r, bool keep) {
+#pragma unroll
+  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) r.w[i] = keep ? r.w[i] : 0u;
+  return r;
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void store8(T* p, int gap, const Raw<T>& r) {
+  if constexpr (kVec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.w);
+      *reinterpret_cast<uint4*>(p + gap) = *reinterpret_cast<const uint4*>(r.w + 4);
+    } else if (gap == 4) {
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.w);
+    } else {
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(r.w);
+      *reinterpret_cast<uint2*>(p + gap) = *reinterpret_cast<const uint2*>(r.w + 2);
     }
   } else {
-    if (vec) {
-      uint2 w[2];
-      T* h = reinterpret_cast<T*>(w);
+    const T* h = reinterpret_cast<const T*>(r.w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = from_f32<T>(f[j]);
-      if (e1 == e0 + 4) {
-        *reinterpret_cast<uint4*>(row + e0) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
-      } else {
-        *reinterpret_cast<uint2*>(row + e0) = w[0];
-        *reinterpret_cast<uint2*>(row + e1) = w[1];
-      }
-      return;
-    }
+    for (int j = 0; j < 4; ++j) p[j] = h[j], p[gap + j] = h[4 + j];
+  }
+}
+
+// Two floats in one 64-bit register pair: one instruction works on both.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum(F2 a, F2 b) {
+  float p, q, r, s;
+  split(a, p, q), split(b, r, s);
+  return (p + q) + (r + s);
+}
+
+// Position in memory (0 .. 7) of value i: values 0 .. 3 are the pairs' first elements, 4 .. 7 their second ones.
+template <bool kPairs>
+__device__ __forceinline__ constexpr int place(int i) {
+  return kPairs ? (i < 4 ? 2 * i : 2 * (i - 4) + 1) : i;
+}
+
+__device__ __forceinline__ void halves(uint32_t w, float& lo, float& hi, __half) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  lo = v.x, hi = v.y;
+}
+__device__ __forceinline__ void halves(uint32_t w, float& lo, float& hi, __nv_bfloat16) {
+  lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t join(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t join(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, bool kPairs>
+__device__ __forceinline__ void unpack(const Raw<T>& r, F2 (&f)[4]) {
+  float m[8];  // in memory's order
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4)
+      m[2 * i] = __uint_as_float(r.w[2 * i]), m[2 * i + 1] = __uint_as_float(r.w[2 * i + 1]);
+    else
+      halves(r.w[i], m[2 * i], m[2 * i + 1], T());
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) row[e0 + j] = from_f32<T>(f[j]), row[e1 + j] = from_f32<T>(f[4 + j]);
+  for (int i = 0; i < 4; ++i) f[i] = f2(m[place<kPairs>(2 * i)], m[place<kPairs>(2 * i + 1)]);
+}
+
+template <typename T, bool kPairs>
+__device__ __forceinline__ Raw<T> pack(const F2 (&f)[4]) {
+  float m[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(f[i], m[place<kPairs>(2 * i)], m[place<kPairs>(2 * i + 1)]);
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4)
+      r.w[2 * i] = __float_as_uint(m[2 * i]), r.w[2 * i + 1] = __float_as_uint(m[2 * i + 1]);
+    else
+      r.w[i] = join(m[2 * i], m[2 * i + 1], T());
+  }
+  return r;
 }
 
 __device__ __forceinline__ double position_at(const void* pos, int dtype, long long i) {
-  if (dtype == kPositionF32) return (double)static_cast<const float*>(pos)[i];
+  if (dtype == kPositionI64) return (double)static_cast<const long long*>(pos)[i];
   if (dtype == kPositionI32) return (double)static_cast<const int*>(pos)[i];
-  return (double)static_cast<const long long*>(pos)[i];
+  return (double)static_cast<const float*>(pos)[i];
 }
 
 // A scale vector's value in any of the three float types.
@@ -101,66 +183,77 @@ __device__ __forceinline__ float scale_at(const void* w, int dtype, int i) {
   return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-// Pairs (j, j + 1) of f for neighbours, (j, j + 4) for split halves, turned by (c, s).
-template <bool kPairs>
-__device__ __forceinline__ void turn(float (&f)[8], const float (&c)[4], const float (&s)[4]) {
+// Pairs (f[0..1], f[2..3]) turned by angles of cosine c and sine s; ns = -s.
+__device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&c)[2], const F2 (&s)[2], const F2 (&ns)[2]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float& a = f[kPairs ? 2 * j : j];
-    float& b = f[kPairs ? 2 * j + 1 : j + 4];
-    const float x = a, y = b;
-    a = x * c[j] - y * s[j];
-    b = x * s[j] + y * c[j];
+  for (int i = 0; i < 2; ++i) {
+    const F2 x = f[i], y = f[2 + i];
+    f[i] = fma2(x, c[i], y * ns[i]);
+    f[2 + i] = fma2(x, s[i], y * c[i]);
   }
 }
 
-template <int G>
-__device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-
-// kBackward: y is dy, x the forward's input (read where the tensor has a
+// kBackward: in is dy, x the forward's input (read where the tensor has a
 // scale), out is dx, and each block leaves its sums of dz xh in partial
 // [block][2][D] (q, then k).
-template <typename T, int G, bool kPairs, bool kBackward>
-__global__ void __launch_bounds__(kWarps * 32) rope_kernel(const __grid_constant__ RopeArgs a) {
+// kVec: every row starts at a multiple of 16 bytes.
+template <typename T, int G, bool kPairs, bool kVec, bool kBackward>
+__global__ void __launch_bounds__(kWarps * 32, kBackward ? 2 : 3) rope_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kRows = 32 / G, kLanePairs = 4 * G;
+  constexpr int kAhead = kBackward ? 2 : 4;  // steps whose rows are in flight at once
+  __shared__ __align__(16) float scales[2][8 * G];
+  __shared__ __align__(16) float cosines[kWarps][kLanePairs], sines[kWarps][kLanePairs];  // of the block's tokens
   __shared__ float sums[kBackward ? kWarps : 1][2][kBackward ? 8 * G : 1];
-  constexpr int kRows = 32 / G;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % G, grp = lane / G;
   const int D = a.D, half = a.pairs;
-  // elements of this lane and its pairs
-  int e0 = 8 * sub, e1 = e0 + 4, p0 = 4 * sub;
-  if (!kPairs && 8 * sub < 2 * half) e0 = 4 * sub, e1 = half + 4 * sub;
+  // this lane's elements are e0 .. e0 + 3 and e0 + gap .. e0 + gap + 3; its pairs 4 sub .. 4 sub + 3
+  const bool apart = !kPairs && 8 * sub < 2 * half;
+  const int e0 = apart ? 4 * sub : 8 * sub, gap = kPairs ? 4 : (apart ? half : 4);
   const bool live = 8 * sub < D;
-  double freq[4];
-  int axis[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool turned = live && p0 + j < half;
-    freq[j] = turned ? a.freq[p0 + j] : 0.0;
-    axis[j] = turned ? (int)a.axis[p0 + j] : 0;
+  for (int i = threadIdx.x; i < 16 * G; i += kWarps * 32) {
+    const int w = i / (8 * G), e = i % (8 * G);
+    scales[w][e] = a.t[w].scale != nullptr && e < D ? scale_at(a.t[w].scale, a.scale_dtype, e) : 0.0f;
   }
-  float dw[2][8];
+  // value i's place in a row that was cut as this lane's elements are
+  auto element = [&](int i) {
+    const int m = place<kPairs>(i);
+    return m < 4 ? e0 + m : e0 + gap + m - 4;
+  };
+  F2 dw[2][4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) dw[0][j] = dw[1][j] = 0.0f;
+  for (int i = 0; i < 4; ++i) dw[0][i] = dw[1][i] = f2(0.0f, 0.0f);
 
-  const long long units = (long long)a.B * a.L * a.parts;
-  for (long long u = (long long)blockIdx.x * kWarps + warp; u < units; u += (long long)gridDim.x * kWarps) {
-    const long long token = u / a.parts;
-    const int part = (int)(u - token * a.parts);
-    const long long b = token / a.L, l = token - b * a.L;
-    float c[4], s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  // this thread's pair of the table; its tokens are threadIdx.x / kLanePairs and so on
+  const int pair = threadIdx.x % kLanePairs;
+  const double freq = pair < half ? a.freq[pair] : 0.0;
+  const long long axis_at = pair < half ? a.axis[pair] * a.pos_stride[2] : 0;
+  const uint32_t tokens = a.tokens, group = a.group;  // tokens a block holds at once: 1, 2, 4 or 8
+  const int slot = warp % group;                      // this warp's token of them
+  const int part = warp / group + (int)blockIdx.y * (kWarps / group);
+
+  for (uint32_t t0 = blockIdx.x * group; t0 < tokens; t0 += gridDim.x * group) {
+    if (kBackward) __syncthreads();  // the last tokens' table is no longer read
+    for (uint32_t i = threadIdx.x / kLanePairs; i < group; i += kWarps * 32 / kLanePairs) {
+      const uint32_t token = min(t0 + i, tokens - 1), b = token / (uint32_t)a.L, l = token - b * (uint32_t)a.L;
       double t = 0.0;
-      if (freq[j] != 0.0)
-        t = position_at(a.pos, a.pos_dtype, b * a.pos_stride[0] + l * a.pos_stride[1] + axis[j] * a.pos_stride[2]) *
-            freq[j];
+      if (pair < half) t = position_at(a.pos, a.pos_dtype, b * a.pos_stride[0] + l * a.pos_stride[1] + axis_at) * freq;
       t -= rint(t);
-      sincospif(2.0f * (float)t, &s[j], &c[j]);
-      if (kBackward) s[j] = -s[j];
+      float sn, cs;
+      sincospif(2.0f * (float)t, &sn, &cs);
+      cosines[i][pair] = cs;
+      sines[i][pair] = kBackward ? -sn : sn;
+    }
+    __syncthreads();
+    const uint32_t token = t0 + slot;
+    if (token >= tokens) continue;
+    const uint32_t bi = token / (uint32_t)a.L;
+    const long long b = bi, l = token - bi * (uint32_t)a.L;
+    F2 c[2], s[2], ns[2];
+    {
+      const float4 cv = *reinterpret_cast<const float4*>(&cosines[slot][4 * sub]);
+      const float4 sv = *reinterpret_cast<const float4*>(&sines[slot][4 * sub]);
+      c[0] = f2(cv.x, cv.y), c[1] = f2(cv.z, cv.w), s[0] = f2(sv.x, sv.y), s[1] = f2(sv.z, sv.w);
+      ns[0] = f2(-sv.x, -sv.y), ns[1] = f2(-sv.z, -sv.w);
     }
     // steps of 32 / G heads: q's, then k's
     const int s0 = part * a.steps_per_part;
@@ -168,61 +261,99 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const __grid_constant
     for (int w = 0; w < 2; ++w) {
       const RopeTensor& x = a.t[w];
       const int first = w ? (a.heads[0] + kRows - 1) / kRows : 0;
+      const int start = max(first, s0);
       const int last = min(first + (a.heads[w] + kRows - 1) / kRows, s0 + a.steps_per_part);
+      if (start >= last) continue;
       const bool norm = x.scale != nullptr;
-      float scale[8];
+      F2 scale[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        scale[j] = norm && live ? scale_at(x.scale, a.scale_dtype, (j < 4 ? e0 : e1 - 4) + j) : 0.0f;
-      for (int step = max(first, s0); step < last; ++step) {
-        const long long h = (step - first) * kRows + grp;
-        const bool row = h < a.heads[w] && live;
-        float f[8], xv[8];
+      for (int i = 0; i < 4; ++i) scale[i] = f2(scales[w][element(2 * i)], scales[w][element(2 * i + 1)]);
+      // this lane's head of the first step, how many of the steps it has a row in, and where that row lies
+      const int h0 = (start - first) * kRows + grp;
+      const int count = live ? min(last - start, (a.heads[w] - h0 + kRows - 1) / kRows) : 0;
+      const T* in0 = static_cast<const T*>(x.in) + b * x.in_stride[0] + l * x.in_stride[2];
+      const T* org0 = static_cast<const T*>(x.x) + b * x.x_stride[0] + l * x.x_stride[2];
+      const T* src = in0 + h0 * x.in_stride[1] + e0;
+      const T* org = org0 + h0 * x.x_stride[1] + e0;
+      T* dst = static_cast<T*>(x.out) + b * x.out_stride[0] + h0 * x.out_stride[1] + l * x.out_stride[2] + e0;
+      const long long src_step = kRows * x.in_stride[1], org_step = kRows * x.x_stride[1];
+      const long long dst_step = kRows * x.out_stride[1];
+      for (int i0 = 0; i0 < last - start; i0 += kAhead) {
+        Raw<T> in[kAhead], xs[kBackward ? kAhead : 1];
+        // a lane without a row reads the token's first head instead, so that no load waits behind a branch
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 0.0f, xv[j] = 0.0f;
-        if (row) {
-          const T* src = static_cast<const T*>(x.in) + b * x.in_stride[0] + h * x.in_stride[1] + l * x.in_stride[2];
-          load8<T>(src, e0, e1, a.vec, f);
-          if (kBackward && norm) {
-            const T* xs = static_cast<const T*>(x.x) + b * x.x_stride[0] + h * x.x_stride[1] + l * x.x_stride[2];
-            load8<T>(xs, e0, e1, a.vec, xv);
+        for (int q = 0; q < kAhead; ++q) {
+          const bool row = i0 + q < count;
+          in[q] = load8<T, kVec>(row ? src : in0, row ? gap : 4);
+          if (kBackward && norm) xs[q] = load8<T, kVec>(row ? org : org0, row ? gap : 4);
+          src += src_step;
+          if (kBackward) org += org_step;
+        }
+        // the rows' sums go through the lanes side by side, so that their shuffles overlap
+        float ss[kAhead], dot[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+          in[q] = masked<T>(in[q], i0 + q < count);
+          ss[q] = dot[q] = 0.0f;
+          if (norm) {
+            F2 xv[4];
+            if constexpr (kBackward) {
+              xs[q] = masked<T>(xs[q], i0 + q < count);
+              F2 t[4];
+              unpack<T, kPairs>(in[q], t);
+              turn(t, c, s, ns);
+              unpack<T, kPairs>(xs[q], xv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t[i] = t[i] * scale[i];
+              dot[q] = sum(fma2(t[1], xv[1], t[0] * xv[0]), fma2(t[3], xv[3], t[2] * xv[2]));
+            } else {
+              unpack<T, kPairs>(in[q], xv);
+            }
+            ss[q] = sum(fma2(xv[1], xv[1], xv[0] * xv[0]), fma2(xv[3], xv[3], xv[2] * xv[2]));
           }
         }
-        if constexpr (!kBackward) {
-          if (norm) {
-            float ss = 0.0f;
+        if (norm) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-            const float r = rsqrtf(row_sum<G>(ss) / (float)D + a.eps);
+          for (int o = G / 2; o > 0; o >>= 1)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = f[j] * r * scale[j];
-          }
-          turn<kPairs>(f, c, s);
-        } else {
-          turn<kPairs>(f, c, s);  // dz
-          if (norm) {
-            float ss = 0.0f, dot = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              ss += xv[j] * xv[j];
-              dot += f[j] * scale[j] * xv[j];
+            for (int q = 0; q < kAhead; ++q) {
+              ss[q] += __shfl_xor_sync(0xFFFFFFFFu, ss[q], o);
+              if (kBackward) dot[q] += __shfl_xor_sync(0xFFFFFFFFu, dot[q], o);
             }
-            const float r = rsqrtf(row_sum<G>(ss) / (float)D + a.eps);
-            const float mean = row_sum<G>(dot) * r / (float)D;  // mean(w dz xh)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float xh = xv[j] * r;
-              dw[w][j] += f[j] * xh;
-              f[j] = r * (f[j] * scale[j] - xh * mean);
-            }
-          }
         }
-        if (row) {
-          T* dst = static_cast<T*>(x.out) + b * x.out_stride[0] + h * x.out_stride[1] + l * x.out_stride[2];
-          store8<T>(dst, e0, e1, a.vec, f);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+          F2 f[4];
+          unpack<T, kPairs>(in[q], f);
+          if (norm) {
+            const float r = rsqrtf(ss[q] * a.inv_dim + a.eps);
+            const F2 rr = f2(r, r);
+            if constexpr (!kBackward) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) f[i] = f[i] * rr * scale[i];
+              turn(f, c, s, ns);
+            } else {
+              turn(f, c, s, ns);  // dz
+              const float mean = dot[q] * r * a.inv_dim;  // mean(w dz xh)
+              const F2 less = f2(-mean, -mean);
+              F2 xv[4];
+              unpack<T, kPairs>(xs[q], xv);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const F2 xh = xv[i] * rr;
+                dw[w][i] = fma2(f[i], xh, dw[w][i]);
+                f[i] = fma2(xh, less, f[i] * scale[i]) * rr;
+              }
+            }
+          } else {
+            turn(f, c, s, ns);
+          }
+          if (i0 + q < count) store8<T, kVec>(dst, gap, pack<T, kPairs>(f));
+          dst += dst_step;
         }
       }
     }
+    if (!kBackward) break;  // one set of tokens a block
   }
   if constexpr (kBackward) {
     if (a.partial == nullptr) return;
@@ -230,92 +361,117 @@ __global__ void __launch_bounds__(kWarps * 32) rope_kernel(const __grid_constant
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = dw[w][j];
+      for (int i = 0; i < 4; ++i) {
+        float v[2];
+        split(dw[w][i], v[0], v[1]);
 #pragma unroll
-        for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        if (grp == 0 && live) sums[warp][w][(j < 4 ? e0 : e1 - 4) + j] = v;
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int o = G; o < 32; o <<= 1) v[j] += __shfl_xor_sync(0xFFFFFFFFu, v[j], o);
+          if (grp == 0 && live) sums[warp][w][element(2 * i + j)] = v[j];
+        }
       }
     __syncthreads();
+    float* out = a.partial + (long long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * D;
     for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
       float v = 0.0f;
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) v += sums[k][i / D][i % D];
-      a.partial[(long long)blockIdx.x * 2 * D + i] = v;
+      out[i] = v;
     }
   }
 }
 
-// dw[t][e] = sum over blocks of partial[block][t][e]: one block per 32 elements, 32 rows of threads.
+// dw[t][e] = sum over blocks of partial[block][t][e], eight columns a block of 8 x 128 threads, in a fixed order.
 __global__ void __launch_bounds__(1024) scale_grad_kernel(const float* partial, int blocks, int D, void* dq, void* dk,
                                                           int dtype) {
-  __shared__ float s[32][33];
-  const int e = blockIdx.x * 32 + threadIdx.x, t = blockIdx.y;
+  __shared__ float s[128][9];
+  const int x = threadIdx.x & 7, y = threadIdx.x >> 3, e = blockIdx.x * 8 + x, t = blockIdx.y;
+  const float* from = partial + (long long)t * D + e;
   float v = 0.0f;
-  if (e < D)
-    for (int b = threadIdx.y; b < blocks; b += 32) v += partial[((long long)b * 2 + t) * D + e];
-  s[threadIdx.y][threadIdx.x] = v;
+#pragma unroll 8
+  for (int b = y; b < blocks; b += 128) v += from[(long long)b * 2 * D];
+  s[y][x] = v;
   __syncthreads();
-  if (threadIdx.y == 0 && e < D) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) sum += s[k][threadIdx.x];
-    void* out = t ? dk : dq;
-    if (out == nullptr) return;
-    if (dtype == GFX_DTYPE_F32)
-      static_cast<float*>(out)[e] = sum;
-    else if (dtype == GFX_DTYPE_F16)
-      static_cast<__half*>(out)[e] = __float2half_rn(sum);
-    else
-      static_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(sum);
+  for (int n = 64; n > 0; n >>= 1) {
+    if (y < n) s[y][x] += s[y + n][x];
+    __syncthreads();
   }
+  void* out = t ? dk : dq;
+  if (y != 0 || out == nullptr) return;
+  if (dtype == GFX_DTYPE_F32)
+    static_cast<float*>(out)[e] = s[0][x];
+  else if (dtype == GFX_DTYPE_F16)
+    static_cast<__half*>(out)[e] = __float2half_rn(s[0][x]);
+  else
+    static_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(s[0][x]);
 }
 
 }  // namespace rotary
 
-// Turns per unit of position of every pair, and the axis that moves it.
+// Turns per unit of position of every pair, and the axis that moves it. Computed again only when the axes or theta
+// are others than the thread's last call had (64 powers take longer than the launch).
 void rope_frequencies(RopeArgs* a, const int* axes_dims, int n_axes, double theta) {
-  int p = 0;
-  for (int i = 0; i < n_axes; ++i)
-    for (int j = 0; j < axes_dims[i] / 2; ++j, ++p) {
-      a->freq[p] = pow(theta, -2.0 * j / axes_dims[i]) / 6.283185307179586476925286766559;
-      a->axis[p] = (unsigned char)i;
-    }
-  a->pairs = p;
+  struct Table {
+    int n = 0, dims[kRopeMaxAxes], pairs;
+    double theta, freq[kRopeMaxDim / 2];
+    unsigned char axis[kRopeMaxDim / 2];
+  };
+  static thread_local Table t;
+  if (t.n != n_axes || t.theta != theta || memcmp(t.dims, axes_dims, sizeof(int) * n_axes) != 0) {
+    int p = 0;
+    for (int i = 0; i < n_axes; ++i)
+      for (int j = 0; j < axes_dims[i] / 2; ++j, ++p) {
+        t.freq[p] = pow(theta, -2.0 * j / axes_dims[i]) / 6.283185307179586476925286766559;
+        t.axis[p] = (unsigned char)i;
+      }
+    t.n = n_axes, t.theta = theta, t.pairs = p;
+    memcpy(t.dims, axes_dims, sizeof(int) * n_axes);
+  }
+  memcpy(a->freq, t.freq, sizeof(double) * t.pairs);
+  memcpy(a->axis, t.axis, t.pairs);
+  a->pairs = t.pairs;
+  a->axes = n_axes;
 }
 
-// Blocks of the launch, and how many parts a token's heads are cut into: a
-// whole token per warp amortises the sines best, but a short sequence is cut
-// until the GPU has two warps for every scheduler or a part is one step.
-static int plan(RopeArgs* a, int rows, int sms) {
+// A block's eight warps hold 8 tokens, or fewer with several warps a token where that leaves less than two waves of
+// blocks; a lone token's heads are spread over blocks too, down to one step a warp. A backward that sums scale
+// gradients keeps to a fixed number of blocks, which walk the tokens.
+static dim3 plan(RopeArgs* a, int rows, int sms) {
   const long long tokens = (long long)a->B * a->L;
   const int steps = (a->heads[0] + rows - 1) / rows + (a->heads[1] + rows - 1) / rows;
-  long long parts = 1;
-  while (parts < steps && tokens * parts < (long long)sms * 8) ++parts;
-  a->steps_per_part = (int)((steps + parts - 1) / parts);
-  a->parts = (steps + a->steps_per_part - 1) / a->steps_per_part;
-  const long long warps = tokens * a->parts, blocks = (warps + rotary::kWarps - 1) / rotary::kWarps;
-  return (int)(blocks < kRopeMaxBlocks ? blocks : kRopeMaxBlocks);
+  int group = rotary::kWarps;
+  while (group > 1 && tokens / group < 6ll * sms) group /= 2;
+  const int warps = rotary::kWarps / group;  // of a token, in one block
+  int spread = 1;
+  while (group == 1 && spread * warps < steps && tokens * spread < sms) ++spread;
+  a->tokens = (unsigned)tokens;
+  a->group = group;
+  a->steps_per_part = (steps + spread * warps - 1) / (spread * warps);
+  const long long blocks = (tokens + group - 1) / group, most = a->partial != nullptr ? kRopeMaxBlocks / spread : blocks;
+  return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)spread);
 }
 
 static int lanes_per_row(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : 32); }
 
-template <typename T, int G, bool kPairs>
-static int launch_t(const RopeArgs& a, bool backward, int blocks, cudaStream_t st) {
+template <typename T, int G, bool kPairs, bool kVec>
+static int launch_t(const RopeArgs& a, bool backward, dim3 blocks, cudaStream_t st) {
   if (backward)
-    rotary::rope_kernel<T, G, kPairs, true><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
+    rotary::rope_kernel<T, G, kPairs, kVec, true><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
   else
-    rotary::rope_kernel<T, G, kPairs, false><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
+    rotary::rope_kernel<T, G, kPairs, kVec, false><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
   return check_launch("rope_kernel");
 }
 
 template <typename T, int G>
-static int launch_p(const RopeArgs& a, bool pairs, bool backward, int blocks, cudaStream_t st) {
-  return pairs ? launch_t<T, G, true>(a, backward, blocks, st) : launch_t<T, G, false>(a, backward, blocks, st);
+static int launch_p(const RopeArgs& a, bool pairs, bool backward, dim3 blocks, cudaStream_t st) {
+  if (a.vec)
+    return pairs ? launch_t<T, G, true, true>(a, backward, blocks, st) : launch_t<T, G, false, true>(a, backward, blocks, st);
+  return pairs ? launch_t<T, G, true, false>(a, backward, blocks, st) : launch_t<T, G, false, false>(a, backward, blocks, st);
 }
 
 template <typename T>
-static int launch_g(const RopeArgs& a, bool pairs, bool backward, int blocks, cudaStream_t st) {
+static int launch_g(const RopeArgs& a, bool pairs, bool backward, dim3 blocks, cudaStream_t st) {
   const int g = lanes_per_row(a.D);
   if (g == 8) return launch_p<T, 8>(a, pairs, backward, blocks, st);
   if (g == 16) return launch_p<T, 16>(a, pairs, backward, blocks, st);
@@ -324,7 +480,7 @@ static int launch_g(const RopeArgs& a, bool pairs, bool backward, int blocks, cu
 
 int launch_rope(RopeArgs& a, int dtype, bool pairs, bool backward, void* dq_scale, void* dk_scale, cudaStream_t st,
                 int sms) {
-  const int blocks = plan(&a, 32 / lanes_per_row(a.D), sms);
+  const dim3 blocks = plan(&a, 32 / lanes_per_row(a.D), sms);
   int rc;
   if (dtype == GFX_DTYPE_F32)
     rc = launch_g<float>(a, pairs, backward, blocks, st);
@@ -333,8 +489,8 @@ int launch_rope(RopeArgs& a, int dtype, bool pairs, bool backward, void* dq_scal
   else
     rc = launch_g<__nv_bfloat16>(a, pairs, backward, blocks, st);
   if (rc || !backward || a.partial == nullptr) return rc;
-  rotary::scale_grad_kernel<<<dim3((a.D + 31) / 32, 2), dim3(32, 32), 0, st>>>(a.partial, blocks, a.D, dq_scale,
-                                                                               dk_scale, a.scale_dtype);
+  rotary::scale_grad_kernel<<<dim3(a.D / 8, 2), 1024, 0, st>>>(a.partial, (int)(blocks.x * blocks.y), a.D, dq_scale,
+                                                               dk_scale, a.scale_dtype);
   return check_launch("scale_grad_kernel");
 }
 

@@ -30,20 +30,25 @@ def _ptr(t: torch.Tensor | None):
     return t.data_ptr() if t is not None else None
 
 
+def _forward(x, w_gate, w_up, b_gate, b_up, act, keep):
+    """(h, the float32 projections that a backward wants: [2, M, F], or None)"""
+    (M, K), N = x.shape, w_gate.shape[0]
+    dev = x.device
+    h = torch.empty((M, N), dtype=x.dtype, device=dev)
+    save = torch.empty((2, M, N), dtype=torch.float32, device=dev) if keep else None
+    with ops._on(dev):
+        stream, need = ops._stream(dev), _lib.load().gated_linear_workspace_bytes(M, K, N)
+        ws = ops._workspace(dev, stream, need)
+        ops._call_gemm("gated_linear", dev, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0),
+                       w_up.data_ptr(), w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._dtype_code(x.dtype), act,
+                       h.data_ptr(), _ptr(save), M, K, N, _ptr(ws), ws.numel() if need else 0, stream)
+    return h, save
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        (M, K), N = x.shape, w_gate.shape[0]
-        h = torch.empty(M, N, dtype=x.dtype, device=x.device)
-        save = None
-        if any(ctx.needs_input_grad[:5]):
-            save = torch.empty(2, M, N, dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
-            stream = ops._stream(x.device)
-            ws = ops._workspace(x.device, stream, _lib.load().gated_linear_workspace_bytes(M, K, N))
-            ops._call_gemm("gated_linear", x.device, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0),
-                           w_up.data_ptr(), w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._dtype_code(x.dtype), act,
-                           h.data_ptr(), _ptr(save), M, K, N, _ptr(ws), ws.numel() if ws is not None else 0, stream)
+        h, save = _forward(x, w_gate, w_up, b_gate, b_up, act, True)
         ctx.act = act
         ctx.save_for_backward(x, w_gate, w_up, save)
         return h
@@ -57,7 +62,7 @@ class _GatedLinear(torch.autograd.Function):
         shapes = ((M, K), (N, K), (N, K), (N,), (N,))
         grads = [torch.empty(s, dtype=x.dtype, device=x.device) if need else None
                  for s, need in zip(shapes, ctx.needs_input_grad)]
-        with torch.cuda.device(x.device):
+        with ops._on(x.device):
             ws = torch.empty(_lib.load().gated_linear_backward_workspace_bytes(M, K, N), dtype=torch.uint8,
                              device=x.device)
             ops._call_gemm("gated_linear_backward", x.device, dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0),
@@ -94,12 +99,16 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     for t, name in ((b_gate, "b_gate"), (b_up, "b_up")):
         if t is not None and tuple(t.shape) != (N,):
             raise RuntimeError(f"{name} must have {N} elements, got {tuple(t.shape)}")
-    x2 = x.reshape(-1, K)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if x2.shape[0] > 2 ** 30:
         raise RuntimeError(f"at most 2^30 tokens, got {x2.shape[0]}")
-    b_gate, b_up = (b.contiguous() if b is not None else None for b in (b_gate, b_up))
-    h = _GatedLinear.apply(_rows(x2), _rows(w_gate), _rows(w_up), b_gate, b_up, ACTIVATIONS[activation])
-    return h.reshape(*x.shape[:-1], N)
+    args = (_rows(x2), _rows(w_gate), _rows(w_up), b_gate.contiguous() if b_gate is not None else None,
+            b_up.contiguous() if b_up is not None else None)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        h = _GatedLinear.apply(*args, ACTIVATIONS[activation])
+    else:
+        h = _forward(*args, ACTIVATIONS[activation], False)[0]
+    return h if x.dim() == 2 else h.reshape(*x.shape[:-1], N)
 
 
 class GatedMLP(torch.nn.Module):

@@ -24,6 +24,7 @@ compute entry point.
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 
 import torch
@@ -36,6 +37,9 @@ ROTATION_SEED = 0
 _DTYPE_CODE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _dtype_code(dt: torch.dtype) -> int:
     try:
         return _DTYPE_CODE[dt]
@@ -44,7 +48,18 @@ def _dtype_code(dt: torch.dtype) -> int:
 
 
 def _stream(device: torch.device) -> int:
+    if _RAW_STREAM is not None and device.index is not None:
+        return _RAW_STREAM(device.index)  # the same handle without building a Stream object (some microseconds)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The context of a call on `device`: nothing to do where it is current, which entering torch.cuda.device would
+    find out in some microseconds."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _require_cuda(t: torch.Tensor, name: str):

@@ -30,53 +30,51 @@ def moment_scales(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-
-
-def _check_lists(params, groups):
-    for name, tensors in groups:
-        if len(tensors) != len(params):
-            raise RuntimeError(f"{name} has {len(tensors)} tensors, params {len(params)}")
-    if not params:
-        return
-    dev, dt, gt = params[0].device, params[0].dtype, groups[0][1][0].dtype
-    ops._dtype_code(dt)
-    ops._dtype_code(gt)
-    ops._require_cuda(params[0], "params[0]")
-    for i, p in enumerate(params):
-        if p.dtype != dt or p.device != dev or not p.is_contiguous():
-            raise RuntimeError(f"params[{i}] must be contiguous, {dt} on {dev} as params[0] is; got {p.dtype} on "
-                               f"{p.device}, strides {p.stride()}")
-
-
-def _check(name, tensors, params, dtype, numel):
-    dev = params[0].device if params else None
-    for i, t in enumerate(tensors):
-        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.numel() != numel(params[i]):
-            raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {numel(params[i])} elements; "
-                               f"got {t.dtype} on {t.device}, {tuple(t.shape)}, strides {t.stride()}")
-
-
-def _grad_scale(grad_scale, params):
-    if grad_scale is None:
-        return None
-    if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != params[0].device:
-        raise RuntimeError(f"grad_scale must be one float32 value on {params[0].device}, got {grad_scale.dtype} "
-                           f"{tuple(grad_scale.shape)} on {grad_scale.device}")
-    return grad_scale.data_ptr()
-
-
-def _call(params, grads, m, v, ms, vs, bits, step, lr, betas, eps, weight_decay, grad_scale):
+def _lists(params, others):
+    """Checks the lists of one step: others is [(name, tensors, dtype or None for the first one's, scales)]; returns
+    (device, elements of each parameter), or None where there is nothing to do. Whole lists are compared at once: a
+    step over many small tensors is bound by this side."""
     n = len(params)
-    scale = _grad_scale(grad_scale, params)
-    numel = (ctypes.c_int64 * n)(*[p.numel() for p in params])
-    with torch.cuda.device(params[0].device):
-        _lib.call("adamw_step", _pointers(params), _pointers(grads), _pointers(m), _pointers(v),
-                  _pointers(ms) if bits == 8 else None, _pointers(vs) if bits == 8 else None, numel, n,
+    for name, tensors, _, _ in others:
+        if len(tensors) != n:
+            raise RuntimeError(f"{name} has {len(tensors)} tensors, params {n}")
+    if n == 0:
+        return None
+    ops._require_cuda(params[0], "params[0]")
+    dev, index, numel = params[0].device, params[0].get_device(), [t.numel() for t in params]
+    ops._dtype_code(params[0].dtype)
+    for name, tensors, dtype, scales in (("params", params, None, False), *others):
+        dtype = dtype or tensors[0].dtype
+        want = [moment_scales(x) for x in numel] if scales else numel
+        wanted = [(dtype, index, x, True) for x in want]
+        got = [(t.dtype, t.get_device(), t.numel(), t.is_contiguous()) for t in tensors]
+        if got != wanted:
+            i = next(i for i in range(n) if got[i] != wanted[i])
+            t = tensors[i]
+            raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {want[i]} elements; got {t.dtype} "
+                               f"on {t.device}, {tuple(t.shape)}, strides {t.stride()}")
+    return dev, numel
+
+
+def _call(dev, numel, lists, bits, step, lr, betas, eps, weight_decay, grad_scale):
+    """lists: params, grads, m, v and, with 8 bits, the moments' scales."""
+    scale = None
+    if grad_scale is not None:
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
+            raise RuntimeError(f"grad_scale must be one float32 value on {dev}, got {grad_scale.dtype} "
+                               f"{tuple(grad_scale.shape)} on {grad_scale.device}")
+        scale = grad_scale.data_ptr()
+    params, grads = lists[:2]
+    n = len(params)
+    # one host array: a row of pointers for each list, then the element counts
+    rows = [t.data_ptr() for x in lists for t in x]
+    table = (ctypes.c_uint64 * (len(rows) + n))(*rows, *numel)
+    at = ctypes.addressof(table)
+    where = [at + 8 * n * i for i in range(len(lists))]
+    with ops._on(dev):
+        _lib.call("adamw_step", *where[:4], *(where[4:] or (None, None)), at + 8 * len(rows), n,
                   ops._dtype_code(params[0].dtype), ops._dtype_code(grads[0].dtype), bits, int(step), float(lr),
-                  float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale,
-                  ops._stream(params[0].device))
+                  float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale, ops._stream(dev))
     torch.autograd.graph.increment_version(params)  # autograd sees the kernel's write as any in-place change
 
 
@@ -89,14 +87,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     float32. ``step`` counts from 1. ``grad_scale`` (one float32 value on the
     device) multiplies every gradient, for clipping or unscaling without a
     pass of its own."""
-    _check_lists(params, [("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)])
-    if not params:
-        return
-    same = torch.Tensor.numel
-    _check("grads", grads, params, grads[0].dtype, same)
-    _check("exp_avgs", exp_avgs, params, torch.float32, same)
-    _check("exp_avg_sqs", exp_avg_sqs, params, torch.float32, same)
-    _call(params, grads, exp_avgs, exp_avg_sqs, None, None, 32, step, lr, betas, eps, weight_decay, grad_scale)
+    found = _lists(params, [("grads", grads, None, False), ("exp_avgs", exp_avgs, torch.float32, False),
+                            ("exp_avg_sqs", exp_avg_sqs, torch.float32, False)])
+    if found:
+        _call(*found, (params, grads, exp_avgs, exp_avg_sqs), 32, step, lr, betas, eps, weight_decay, grad_scale)
 
 
 def adamw_step_8bit(params, grads, m_codes, m_scales, v_codes, v_scales, *, step: int, lr: float, betas=(0.9, 0.999),
@@ -105,21 +99,12 @@ def adamw_step_8bit(params, grads, m_codes, m_scales, v_codes, v_scales, *, step
     with a tensor's elements, m_scales and v_scales float32 with one value per
     256 elements (``moment_scales``). Zeros are a fresh state. The parameters
     move by the moments as computed, before they are rounded to codes."""
-    _check_lists(params, [("grads", grads), ("m_codes", m_codes), ("m_scales", m_scales), ("v_codes", v_codes),
-                          ("v_scales", v_scales)])
-    if not params:
-        return
-    same = torch.Tensor.numel
-
-    def scales(p):
-        return moment_scales(p.numel())
-
-    _check("grads", grads, params, grads[0].dtype, same)
-    _check("m_codes", m_codes, params, torch.int8, same)
-    _check("v_codes", v_codes, params, torch.uint8, same)
-    _check("m_scales", m_scales, params, torch.float32, scales)
-    _check("v_scales", v_scales, params, torch.float32, scales)
-    _call(params, grads, m_codes, v_codes, m_scales, v_scales, 8, step, lr, betas, eps, weight_decay, grad_scale)
+    found = _lists(params, [("grads", grads, None, False), ("m_codes", m_codes, torch.int8, False),
+                            ("v_codes", v_codes, torch.uint8, False), ("m_scales", m_scales, torch.float32, True),
+                            ("v_scales", v_scales, torch.float32, True)])
+    if found:
+        _call(*found, (params, grads, m_codes, v_codes, m_scales, v_scales), 8, step, lr, betas, eps, weight_decay,
+              grad_scale)
 
 
 def moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
@@ -133,7 +118,7 @@ def moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
                            f"{scales.dtype} {tuple(scales.shape)} on {scales.device}")
     c, s = codes.contiguous(), scales.contiguous()
     out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
-    with torch.cuda.device(codes.device):
+    with ops._on(codes.device):
         _lib.call("adamw_moment_values", c.data_ptr(), s.data_ptr(), out.data_ptr(), c.numel(),
                   int(codes.dtype == torch.uint8), ops._stream(codes.device))
     return out

@@ -10,6 +10,7 @@ and writes the [B, H, L, D] layout that attention takes.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -19,8 +20,23 @@ from . import _lib, ops
 _POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 
-def _strides(t: torch.Tensor | None):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3]) if t is not None else None
+@functools.lru_cache(maxsize=64)
+def _axes(dims: tuple):
+    return (ctypes.c_int * len(dims))(*[int(d) for d in dims])
+
+
+def _strides(*lists):
+    """One int64 array of three strides for each list, and the address of each."""
+    flat = (ctypes.c_int64 * (3 * len(lists)))(*[s for x in lists for s in x[:3]])
+    at = ctypes.addressof(flat)
+    return flat, range(at, at + 24 * len(lists), 24)
+
+
+_NONE = (0, 0, 0)
+
+
+def _of(t: torch.Tensor | None):
+    return t.stride() if t is not None else _NONE
 
 
 def _ptr(t: torch.Tensor | None):
@@ -41,45 +57,48 @@ def _like_tokens(x: torch.Tensor) -> torch.Tensor:
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _forward(q, k, positions, pos_strides, q_scale, k_scale, call):
+    B, H, L, D = q.shape
+    dev, code, scale_code, kv, tail = q.device, *call
+    q_out = torch.empty((B, H, L, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((B, kv, L, D), dtype=q.dtype, device=dev) if k is not None else None
+    keep, (qs, ks, ps, qos, kos) = _strides(q.stride(), _of(k), pos_strides, q_out.stride(), _of(k_out))
+    with ops._on(dev):
+        _lib.call("qk_norm_rope", q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(),
+                  _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale), scale_code, q_out.data_ptr(), qos,
+                  _ptr(k_out), kos, B, H, kv, L, D, *tail, ops._stream(dev))
+    return q_out, k_out
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, q_scale, k_scale, axes, theta, eps, interleaved):
-        B, H, L, D = q.shape
-        q_out = torch.empty(B, H, L, D, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k is not None else None
-        scale = q_scale if q_scale is not None else k_scale
-        code = ops._dtype_code(q.dtype)
-        ctx.tail = (B, H, k.shape[1] if k is not None else 0, L, D, axes, len(axes), float(theta), int(interleaved),
-                    float(eps))
-        ctx.pos_args = (_POSITIONS[positions.dtype], (ctypes.c_int64 * 3)(*positions.stride()))
-        ctx.codes = (code, ops._dtype_code(scale.dtype) if scale is not None else code)
-        with torch.cuda.device(q.device):
-            _lib.call("qk_norm_rope", q.data_ptr(), _strides(q), _ptr(k), _strides(k), code, positions.data_ptr(),
-                      *ctx.pos_args, _ptr(q_scale), _ptr(k_scale), ctx.codes[1], q_out.data_ptr(), _strides(q_out),
-                      _ptr(k_out), _strides(k_out), *ctx.tail, ops._stream(q.device))
+    def forward(ctx, q, k, positions, q_scale, k_scale, pos_strides, call):
+        ctx.pos_strides, ctx.call = pos_strides, call
         ctx.save_for_backward(q, k, positions, q_scale, k_scale)
-        return q_out, k_out
+        return _forward(q, k, positions, pos_strides, q_scale, k_scale, call)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, positions, q_scale, k_scale = ctx.saved_tensors
-        B, H, Hk, L, D = ctx.tail[:5]
+        B, H, L, D = q.shape
+        dev, code, scale_code, kv, tail = q.device, *ctx.call
         dq_out = _rows(dq_out)
         dk_out = _rows(dk_out) if k is not None else None
         dq, dk = _like_tokens(q), _like_tokens(k) if k is not None else None
         dqs = torch.empty_like(q_scale) if q_scale is not None and ctx.needs_input_grad[3] else None
         dks = torch.empty_like(k_scale) if k_scale is not None and ctx.needs_input_grad[4] else None
-        with torch.cuda.device(q.device):
+        keep, (dqo, dko, qs, ks, ps, dqi, dki) = _strides(dq_out.stride(), _of(dk_out), q.stride(), _of(k),
+                                                          ctx.pos_strides, dq.stride(), _of(dk))
+        with ops._on(dev):
             ws = None
             if dqs is not None or dks is not None:
-                ws = torch.empty(_lib.load().qk_norm_rope_workspace_bytes(D), dtype=torch.uint8, device=q.device)
-            _lib.call("qk_norm_rope_backward", dq_out.data_ptr(), _strides(dq_out), _ptr(dk_out), _strides(dk_out),
-                      q.data_ptr(), _strides(q), _ptr(k), _strides(k), ctx.codes[0], positions.data_ptr(),
-                      *ctx.pos_args, _ptr(q_scale), _ptr(k_scale), ctx.codes[1], dq.data_ptr(), _strides(dq),
-                      _ptr(dk), _strides(dk), _ptr(dqs), _ptr(dks), *ctx.tail, _ptr(ws),
-                      ws.numel() if ws is not None else 0, ops._stream(q.device))
-        return dq, dk, None, dqs, dks, None, None, None, None
+                ws = torch.empty(_lib.load().qk_norm_rope_workspace_bytes(D), dtype=torch.uint8, device=dev)
+            _lib.call("qk_norm_rope_backward", dq_out.data_ptr(), dqo, _ptr(dk_out), dko, q.data_ptr(), qs, _ptr(k),
+                      ks, code, positions.data_ptr(), _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale),
+                      scale_code, dq.data_ptr(), dqi, _ptr(dk), dki, _ptr(dqs), _ptr(dks), B, H, kv, L, D, *tail,
+                      _ptr(ws), ws.numel() if ws is not None else 0, ops._stream(dev))
+        return dq, dk, None, dqs, dks, None, None
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dims, theta: float = 10000.0,
@@ -98,38 +117,43 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     i + sum(axes_dims) / 2. Pair j of an axis of d elements turns by
     position * theta^(-2j/d). q_scale / k_scale [D]: the norm's scale (None:
     that tensor is not normalised). Differentiable in q, k and the scales."""
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None:
-            continue
-        ops._require_cuda(t, name)
-        ops._dtype_code(t.dtype)
-        if t.dim() != 4:
-            raise RuntimeError(f"{name} must be [B, H, L, D], got {tuple(t.shape)}")
-    B, _, L, D = q.shape
-    if k is not None and (k.shape[0] != B or k.shape[2] != L or k.shape[3] != D or k.dtype != q.dtype
-                          or k.device != q.device):
-        raise RuntimeError(f"k must be {q.dtype} [{B}, KVH, {L}, {D}] on {q.device}, got {k.dtype} {tuple(k.shape)} on "
-                           f"{k.device}")
-    axes = tuple(int(d) for d in axes_dims)
+    ops._require_cuda(q, "q")
+    code = ops._dtype_code(q.dtype)
+    if q.dim() != 4:
+        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(q.shape)}")
+    dev, (B, _, L, D) = q.device, q.shape
+    kv = 0
+    if k is not None:
+        if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:] or k.dtype != q.dtype or k.device != dev:
+            raise RuntimeError(f"k must be {q.dtype} [{B}, KVH, {L}, {D}] on {dev}, got {k.dtype} {tuple(k.shape)} on "
+                               f"{k.device}")
+        kv = k.shape[1]
+    elif k_scale is not None:
+        raise RuntimeError("k_scale without k")
+    axes = _axes(tuple(axes_dims))
+    n = len(axes)
     if positions.dtype not in _POSITIONS:
         raise RuntimeError(f"positions must be float32, int32 or int64, got {positions.dtype}")
-    if positions.device != q.device:
-        raise RuntimeError(f"positions must be on {q.device}, got {positions.device}")
-    if positions.dim() == 2:
-        positions = positions[None]
-    if positions.dim() != 3 or positions.shape[0] not in (1, B) or tuple(positions.shape[1:]) != (L, len(axes)):
-        raise RuntimeError(f"positions must be [{L}, {len(axes)}] or [{B}, {L}, {len(axes)}], got "
-                           f"{tuple(positions.shape)}")
-    positions = positions.expand(B, L, len(axes))
-    scales = [s for s in (q_scale, k_scale) if s is not None]
-    for s in scales:
-        if s.numel() != D or s.dtype != scales[0].dtype or s.device != q.device:
-            raise RuntimeError(f"scales must be [{D}] of one dtype on {q.device}, got {s.dtype} {tuple(s.shape)} on "
-                               f"{s.device}")
-        ops._dtype_code(s.dtype)
-    if k is None and k_scale is not None:
-        raise RuntimeError("k_scale without k")
-    q, k = _rows(q), _rows(k) if k is not None else None
-    q_scale, k_scale = (s.contiguous() if s is not None else None for s in (q_scale, k_scale))
-    return _QkNormRope.apply(q, k, positions, q_scale, k_scale, (ctypes.c_int * len(axes))(*axes), theta, eps,
-                             interleaved)
+    if positions.device != dev:
+        raise RuntimeError(f"positions must be on {dev}, got {positions.device}")
+    shape, ps = tuple(positions.shape), positions.stride()
+    if shape == (L, n):
+        ps = (0, *ps)
+    elif shape == (1, L, n):
+        ps = (0, ps[1], ps[2])
+    elif shape != (B, L, n):
+        raise RuntimeError(f"positions must be [{L}, {n}] or [{B}, {L}, {n}], got {shape}")
+    scale_code = code
+    first = q_scale if q_scale is not None else k_scale
+    if first is not None:
+        for s in (q_scale, k_scale):
+            if s is not None and (s.numel() != D or s.dtype != first.dtype or s.device != dev):
+                raise RuntimeError(f"scales must be [{D}] of one dtype on {dev}, got {s.dtype} {tuple(s.shape)} on "
+                                   f"{s.device}")
+        scale_code = ops._dtype_code(first.dtype)
+        q_scale, k_scale = (s.contiguous() if s is not None else None for s in (q_scale, k_scale))
+    args = (_rows(q), _rows(k) if k is not None else None, positions, ps, q_scale, k_scale)
+    call = (code, scale_code, kv, (axes, n, float(theta), int(interleaved), float(eps)))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_scale, k_scale)):
+        return _QkNormRope.apply(*args[:3], *args[4:], ps, call)
+    return _forward(*args, call)

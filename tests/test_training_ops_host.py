@@ -54,7 +54,8 @@ def _rope(lib, back=False, q=16, k=16, dt=2, pos=16, pdt=1, qs=16, ks=16, sdt=2,
 
 @pytest.mark.parametrize("kw,code,needle", [
     (dict(dt=3), INVALID, "dtype"), (dict(sdt=7), INVALID, "dtype"), (dict(pdt=3), INVALID, "positions"),
-    (dict(B=-1), INVALID, "B=-1"), (dict(D=20), UNSUPPORTED, "multiple of 8"), (dict(D=264), UNSUPPORTED, "up to 256"),
+    (dict(B=-1), INVALID, "B=-1"), (dict(B=1 << 20, L=1 << 11), UNSUPPORTED, "2^30 tokens"),
+    (dict(Hk=1 << 21), UNSUPPORTED, "2^20 heads"), (dict(D=20), UNSUPPORTED, "multiple of 8"), (dict(D=264), UNSUPPORTED, "up to 256"),
     (dict(axes=None), INVALID, "axes"), (dict(axes=(2,) * 9), INVALID, "between 1 and 8"),
     (dict(axes=(5,)), INVALID, "even"), (dict(axes=(0, 64)), INVALID, "even"), (dict(axes=(64, 2)), INVALID, "add up"),
     (dict(axes=(2 ** 30, 2 ** 30, 2 ** 30, 2 ** 30)), INVALID, "add up"),
