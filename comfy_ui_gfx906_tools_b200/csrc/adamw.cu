@@ -14,11 +14,21 @@
 // is computed.
 //
 // Memory-bound: p is read and written, g read, each moment read and written.
-// A warp owns 256 consecutive elements, which is one block of the 8-bit form:
-// its largest magnitude is one warp-wide integer maximum (magnitudes order as
-// their bit patterns do, and a NaN lies above every number, so it is not lost).
-// A lane holds elements 4 l .. 4 l + 3 of each 128-element half, so every
-// access of the warp is one contiguous run.
+// A warp owns 256 consecutive elements at a time, which is one block of the
+// 8-bit form: its largest magnitude is one warp-wide integer maximum
+// (magnitudes order as their bit patterns do, and a NaN lies above every
+// number, so it is not lost). A lane holds elements 4 l .. 4 l + 3 of each
+// 128-element half, so every access of the warp is one contiguous run.
+//
+// With 8-bit moments the arithmetic would take longer than the memory if every
+// root were correctly rounded (100 instructions an element, 758 us for 151 M
+// bfloat16 elements against 232 us of memory). The full blocks' path takes the
+// hardware's approximate roots, off by some 2^-22, and decides a code by them
+// unless the root lies within 2.5e-4 of the middle between two codes, where
+// that error could matter; a lane that sees such an element (one in two
+// thousand), or a vanishing root, does its eight elements again exactly. Codes
+// are turned into floats and back by adding 2^23 and 1.5 * 2^23, not by the
+// quarter-rate conversions.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -134,6 +144,238 @@ __device__ __forceinline__ uint32_t code_of(float magnitude, float inv, int top)
   return (uint32_t)min(__float2int_rn(__fsqrt_rn(__fmul_rn(magnitude, inv))), top);
 }
 
+// Four int8 codes (as offset binary) or uint8 codes as floats: the bytes become the low end of 2^23 + u.
+__device__ __forceinline__ float code_float(uint32_t w, int j, float offset) {
+  return __uint_as_float(prmt(w, 0x4B000000u, 0x7650u & ~0xFu | (uint32_t)j)) - offset;
+}
+
+__device__ __forceinline__ float root_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  const uint32_t lo = prmt(__float_as_uint(a), __float_as_uint(b), 0x0040u);
+  const uint32_t hi = prmt(__float_as_uint(c), __float_as_uint(d), 0x0040u);
+  return prmt(lo, hi, 0x5410u);
+}
+
+constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, whose low byte is the code
+constexpr float kNearTie = 0.5f - 2.5e-4f;
+
+// m and v of one element after the step
+__device__ __forceinline__ void moments(const Args& a, float g, float& m, float& v) {
+  m = __fadd_rn(__fmul_rn(m, a.beta1), __fmul_rn(g, a.one_minus_beta1));
+  v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), a.one_minus_beta2));
+}
+
+__device__ __forceinline__ float moved(const Args& a, float p, float m, float root) {
+  return p * a.decay - a.step_size * (m / (root * a.root_scale + a.eps));
+}
+
+// The exact codes of four elements (first moments as int8, roots as uint8).
+__device__ __forceinline__ void exact_codes(const float (&m)[4], const float (&root)[4], float mi, float vi,
+                                            uint32_t& mw, uint32_t& vw) {
+  mw = vw = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = (int)code_of(fabsf(m[j]), mi, 127);
+    mw |= ((uint32_t)(m[j] < 0.0f ? -c : c) & 0xFFu) << (8 * j);
+    uint32_t d = code_of(root[j], vi, 255);
+    if (vi > 0.0f && root[j] > 0.0f && d == 0) d = 1;
+    vw |= d << (8 * j);
+  }
+}
+
+// A block of 256 whose elements all exist and whose arrays are aligned, 8-bit moments.
+template <typename P, typename G>
+__device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t, long long b, int lane, float gs) {
+  const long long e = b * kBlock + lane * 4;
+  typename Quad<P>::V pv[2];
+  typename Quad<G>::V gv[2];
+  uint32_t mc[2], vc[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pv[h] = *reinterpret_cast<const typename Quad<P>::V*>(static_cast<const P*>(t.p) + e + 128 * h);
+    gv[h] = *reinterpret_cast<const typename Quad<G>::V*>(static_cast<const G*>(t.g) + e + 128 * h);
+    mc[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + e + 128 * h);
+    vc[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + e + 128 * h);
+  }
+  const float ms = t.m_scale[b], vs = t.v_scale[b];
+  float m[2][4], v[2][4], root[2][4];
+  uint32_t mb = 0, vb = 0;
+  float least = 1.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float g[4];
+    Quad<G>::unpack(gv[h], g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float c = code_float(mc[h] ^ 0x80808080u, j, 8388736.0f), d = code_float(vc[h], j, 8388608.0f);
+      const float r = __fmul_rn(d * d, vs);
+      m[h][j] = __fmul_rn(c * fabsf(c), ms);
+      v[h][j] = __fmul_rn(r, r);
+      moments(a, __fmul_rn(g[j], gs), m[h][j], v[h][j]);
+      mb = max(mb, __float_as_uint(m[h][j]) & 0x7FFFFFFFu);
+      vb = max(vb, __float_as_uint(v[h][j]));
+      root[h][j] = root_approx(v[h][j]);
+      least = fminf(least, root[h][j]);
+    }
+  }
+  mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+  vb = __reduce_max_sync(0xFFFFFFFFu, vb);  // of the values: the root of the largest is the largest root
+  float mi, vi;
+  const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi);
+  const float vs1 = block_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(vb))), 1.0f / 65025.0f, vi);
+  float far = 0.0f;  // the largest distance of a root from its code
+  uint32_t mw[2], vw[2];
+  float p[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float r[4], q[4];
+    Quad<P>::unpack(pv[h], p[h]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = copysignf(root_approx(fabsf(m[h][j]) * mi), m[h][j]), y = root_approx(root[h][j] * vi);
+      r[j] = x + kRound, q[j] = y + kRound;
+      far = fmaxf(far, fmaxf(fabsf(x - (r[j] - kRound)), fabsf(y - (q[j] - kRound))));
+      q[j] = fmaxf(q[j], kRound + 1.0f);  // a vanishing root goes the exact way
+      p[h][j] = p[h][j] * a.decay - a.step_size * __fdividef(m[h][j], root[h][j] * a.root_scale + a.eps);
+    }
+    mw[h] = low_bytes(r[0], r[1], r[2], r[3]);
+    vw[h] = low_bytes(q[0], q[1], q[2], q[3]);
+  }
+  if (!(far < kNearTie) || !(least > 0.0f) || mi == 0.0f || vi == 0.0f) {
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      float exact[4], mh[4], ph[4];
+      const typename Quad<P>::V old = h ? pv[1] : pv[0];
+      Quad<P>::unpack(old, ph);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mh[j] = h ? m[1][j] : m[0][j];
+        exact[j] = __fsqrt_rn(h ? v[1][j] : v[0][j]);
+        ph[j] = moved(a, ph[j], mh[j], exact[j]);
+      }
+      uint32_t x, y;
+      exact_codes(mh, exact, mi, vi, x, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (h) p[1][j] = ph[j]; else p[0][j] = ph[j];
+      if (h) mw[1] = x, vw[1] = y; else mw[0] = x, vw[0] = y;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = Quad<P>::pack(p[h]);
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + e + 128 * h) = mw[h];
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + e + 128 * h) = vw[h];
+  }
+  if (lane == 0) {
+    t.m_scale[b] = ms1;
+    t.v_scale[b] = vs1;
+  }
+}
+
+// The same with 32-bit moments.
+template <typename P, typename G>
+__device__ __forceinline__ void full_block32(const Args& a, const AdamwTensor& t, long long b, int lane, float gs) {
+  const long long e = b * kBlock + lane * 4;
+  typename Quad<P>::V pv[2];
+  typename Quad<G>::V gv[2];
+  float4 mv[2], vv[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pv[h] = *reinterpret_cast<const typename Quad<P>::V*>(static_cast<const P*>(t.p) + e + 128 * h);
+    gv[h] = *reinterpret_cast<const typename Quad<G>::V*>(static_cast<const G*>(t.g) + e + 128 * h);
+    mv[h] = *reinterpret_cast<const float4*>(static_cast<const float*>(t.m) + e + 128 * h);
+    vv[h] = *reinterpret_cast<const float4*>(static_cast<const float*>(t.v) + e + 128 * h);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float p[4], g[4], m[4], v[4];
+    Quad<P>::unpack(pv[h], p);
+    Quad<G>::unpack(gv[h], g);
+    Quad<float>::unpack(mv[h], m);
+    Quad<float>::unpack(vv[h], v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      moments(a, __fmul_rn(g[j], gs), m[j], v[j]);
+      p[j] = moved(a, p[j], m[j], __fsqrt_rn(v[j]));
+    }
+    *reinterpret_cast<float4*>(static_cast<float*>(t.m) + e + 128 * h) = Quad<float>::pack(m);
+    *reinterpret_cast<float4*>(static_cast<float*>(t.v) + e + 128 * h) = Quad<float>::pack(v);
+    *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = Quad<P>::pack(p);
+  }
+}
+
+// A block that ends a tensor, or whose arrays are not aligned.
+template <typename P, typename G, bool k8>
+__device__ __noinline__ void ragged_block(const Args& a, const AdamwTensor& t, long long b, int lane, float gs) {
+  const long long n = t.n;
+  const bool vec = t.aligned != 0;
+  float m[2][4], v[2][4];
+  const float ms = k8 ? t.m_scale[b] : 0.0f, vs = k8 ? t.v_scale[b] : 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long long e = b * kBlock + h * 128 + lane * 4;
+    float p[4], g[4];
+    load4<P>(t.p, e, n, vec, p);
+    load4<G>(t.g, e, n, vec, g);
+    if constexpr (k8) {
+      const uint32_t mw = load_codes(t.m, e, n, vec), vw = load_codes(t.v, e, n, vec);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[h][j] = first_value(mw, j, ms);
+        const float r = root_value(vw, j, vs);
+        v[h][j] = __fmul_rn(r, r);
+      }
+    } else {
+      load4<float>(t.m, e, n, vec, m[h]);
+      load4<float>(t.v, e, n, vec, v[h]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) moments(a, __fmul_rn(g[j], gs), m[h][j], v[h][j]);
+    if constexpr (!k8) {
+      store4<float>(t.m, e, n, vec, m[h]);
+      store4<float>(t.v, e, n, vec, v[h]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[h][j] = __fsqrt_rn(v[h][j]);
+      p[j] = moved(a, p[j], m[h][j], v[h][j]);
+    }
+    store4<P>(t.p, e, n, vec, p);
+  }
+  if constexpr (k8) {
+    uint32_t mb = 0, vb = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mb = max(mb, __float_as_uint(m[h][j]) & 0x7FFFFFFFu);
+        vb = max(vb, __float_as_uint(v[h][j]) & 0x7FFFFFFFu);
+      }
+    mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+    vb = __reduce_max_sync(0xFFFFFFFFu, vb);
+    float mi, vi;
+    const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi), vs1 = block_scale(vb, 1.0f / 65025.0f, vi);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long e = b * kBlock + h * 128 + lane * 4;
+      uint32_t mw, vw;
+      exact_codes(m[h], v[h], mi, vi, mw, vw);
+      store_codes(t.m, e, n, vec, mw);
+      store_codes(t.v, e, n, vec, vw);
+    }
+    if (lane == 0) {
+      t.m_scale[b] = ms1;
+      t.v_scale[b] = vs1;
+    }
+  }
+}
+
 template <typename P, typename G, bool k8>
 __global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ Args a) {
   // the tensor of this CTA: the last whose first CTA is not past it
@@ -147,79 +389,13 @@ __global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constan
   const long long b0 = (long long)((int)blockIdx.x - t.first_cta) * a.blocks_per_cta;
   const long long b1 = b0 + a.blocks_per_cta < blocks ? b0 + a.blocks_per_cta : blocks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool vec = t.aligned != 0;
   const float gs = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
-
   for (long long b = b0 + warp; b < b1; b += kWarps) {
-    float m[2][4], v[2][4], p[2][4];
-    const float ms = k8 ? t.m_scale[b] : 0.0f, vs = k8 ? t.v_scale[b] : 0.0f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long long e = b * kBlock + h * 128 + lane * 4;
-      float g[4];
-      load4<P>(t.p, e, n, vec, p[h]);
-      load4<G>(t.g, e, n, vec, g);
-      if constexpr (k8) {
-        const uint32_t mw = load_codes(t.m, e, n, vec), vw = load_codes(t.v, e, n, vec);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          m[h][j] = first_value(mw, j, ms);
-          const float r = root_value(vw, j, vs);
-          v[h][j] = __fmul_rn(r, r);
-        }
-      } else {
-        load4<float>(t.m, e, n, vec, m[h]);
-        load4<float>(t.v, e, n, vec, v[h]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float gj = __fmul_rn(g[j], gs);
-        m[h][j] = __fadd_rn(__fmul_rn(m[h][j], a.beta1), __fmul_rn(gj, a.one_minus_beta1));
-        v[h][j] = __fadd_rn(__fmul_rn(v[h][j], a.beta2), __fmul_rn(__fmul_rn(gj, gj), a.one_minus_beta2));
-      }
-      if constexpr (!k8) {
-        store4<float>(t.m, e, n, vec, m[h]);
-        store4<float>(t.v, e, n, vec, v[h]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[h][j] = __fsqrt_rn(v[h][j]);
-        p[h][j] = p[h][j] * a.decay - a.step_size * (m[h][j] / (v[h][j] * a.root_scale + a.eps));
-      }
-      store4<P>(t.p, e, n, vec, p[h]);
-    }
-    if constexpr (k8) {
-      uint32_t mb = 0, vb = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mb = max(mb, __float_as_uint(m[h][j]) & 0x7FFFFFFFu);
-          vb = max(vb, __float_as_uint(v[h][j]) & 0x7FFFFFFFu);
-        }
-      mb = __reduce_max_sync(0xFFFFFFFFu, mb);
-      vb = __reduce_max_sync(0xFFFFFFFFu, vb);
-      float mi, vi;
-      const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi), vs1 = block_scale(vb, 1.0f / 65025.0f, vi);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long e = b * kBlock + h * 128 + lane * 4;
-        uint32_t mw = 0, vw = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = (int)code_of(fabsf(m[h][j]), mi, 127);
-          mw |= ((uint32_t)(m[h][j] < 0.0f ? -c : c) & 0xFFu) << (8 * j);
-          uint32_t d = code_of(v[h][j], vi, 255);
-          if (vi > 0.0f && v[h][j] > 0.0f && d == 0) d = 1;
-          vw |= d << (8 * j);
-        }
-        store_codes(t.m, e, n, vec, mw);
-        store_codes(t.v, e, n, vec, vw);
-      }
-      if (lane == 0) {
-        t.m_scale[b] = ms1;
-        t.v_scale[b] = vs1;
-      }
+    if (t.aligned != 0 && (b + 1) * kBlock <= n) {
+      if constexpr (k8) full_block8<P, G>(a, t, b, lane, gs);
+      else full_block32<P, G>(a, t, b, lane, gs);
+    } else {
+      ragged_block<P, G, k8>(a, t, b, lane, gs);
     }
   }
 }
@@ -230,20 +406,30 @@ __global__ void __launch_bounds__(kWarps * 32) moment_values_kernel(const void* 
                                                                     long long n, int vec) {
   const int lane = threadIdx.x & 31;
   const long long blocks = (n + kBlock - 1) / kBlock;
-  for (long long b = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); b < blocks; b += (long long)gridDim.x * kWarps) {
-    const float s = scale[b];
+  constexpr int kAhead = 4;  // blocks whose codes are in flight at once
+  const long long stride = (long long)gridDim.x * kWarps;
+  for (long long b = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); b < blocks; b += kAhead * stride) {
+    uint32_t w[kAhead][2];
+    float s[kAhead];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long long e = b * kBlock + h * 128 + lane * 4;
-      const uint32_t w = load_codes(codes, e, n, vec != 0);
-      float f[4];
+    for (int q = 0; q < kAhead; ++q) {
+      const long long bq = b + q * stride;
+      s[q] = bq < blocks ? scale[bq] : 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[j] = kSecond ? root_value(w, j, s) : first_value(w, j, s);
-        if (kSecond) f[j] = __fmul_rn(f[j], f[j]);
-      }
-      store4<float>(out, e, n, vec != 0, f);
+      for (int h = 0; h < 2; ++h) w[q][h] = load_codes(codes, bq * kBlock + h * 128 + lane * 4, n, vec != 0);
     }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[j] = kSecond ? root_value(w[q][h], j, s[q]) : first_value(w[q][h], j, s[q]);
+          if (kSecond) f[j] = __fmul_rn(f[j], f[j]);
+        }
+        store4<float>(out, (b + q * stride) * kBlock + h * 128 + lane * 4, n, vec != 0, f);
+      }
   }
 }
 
@@ -271,8 +457,11 @@ int launch_adamw(const AdamwTensor* tensors, int count, int p_dtype, int g_dtype
   a.grad_scale = c.grad_scale;
   a.beta1 = c.beta1, a.one_minus_beta1 = c.one_minus_beta1, a.beta2 = c.beta2, a.one_minus_beta2 = c.one_minus_beta2;
   a.decay = c.decay, a.step_size = c.step_size, a.root_scale = c.root_scale, a.eps = c.eps;
-  (void)sms;
-  a.blocks_per_cta = adamw::kWarps;
+  // one 256-element block a warp where that is needed to fill the GPU, up to four, which amortise a CTA's start
+  long long all = 0;
+  for (int i = 0; i < count; ++i) all += (tensors[i].n + adamw::kBlock - 1) / adamw::kBlock;
+  const long long per_warp = all / ((long long)sms * 48);
+  a.blocks_per_cta = adamw::kWarps * (int)(per_warp < 1 ? 1 : (per_warp > 4 ? 4 : per_warp));
   for (int i = 0; i < count;) {
     // as many tensors as one launch's arguments hold; empty ones take no CTA
     a.count = 0;
