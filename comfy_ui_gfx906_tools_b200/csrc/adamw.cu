@@ -23,12 +23,12 @@
 // With 8-bit moments the arithmetic would take longer than the memory if every
 // root were correctly rounded (100 instructions an element, 758 us for 151 M
 // bfloat16 elements against 232 us of memory). The full blocks' path takes the
-// hardware's approximate roots, off by some 2^-22, and decides a code by them
-// unless the root lies within 2.5e-4 of the middle between two codes, where
-// that error could matter; a lane that sees such an element (one in two
-// thousand), or a vanishing root, does its eight elements again exactly. Codes
-// are turned into floats and back by adding 2^23 and 1.5 * 2^23, not by the
-// quarter-rate conversions.
+// hardware's approximate roots, off by 2^-23, and decides a code by them unless
+// the root lies so near the middle between two codes that this error could
+// matter; a lane that sees such an element (one in five thousand), or a
+// vanishing root, does its eight elements again exactly. Codes are turned into
+// floats and back by adding 2^23 and 1.5 * 2^23, not by the quarter-rate
+// conversions.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -136,7 +136,7 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits, float over, flo
   inv = 0.0f;
   if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
   if (s < 1.17549435e-38f) return 0.0f;
-  inv = __fdiv_rn(1.0f, s);
+  inv = __frcp_rn(s);
   return s;
 }
 
@@ -155,6 +155,12 @@ __device__ __forceinline__ float root_approx(float x) {
   return r;
 }
 
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
   const uint32_t lo = prmt(__float_as_uint(a), __float_as_uint(b), 0x0040u);
   const uint32_t hi = prmt(__float_as_uint(c), __float_as_uint(d), 0x0040u);
@@ -162,7 +168,10 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 }
 
 constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, whose low byte is the code
-constexpr float kNearTie = 0.5f - 2.5e-4f;
+// How near the middle between two codes a root may come before it is taken exactly. An approximate root is off by 2^-23
+// of itself: a first moment's (up to 127) differs from the exact one by at most 1.5 * 2^-23, a second's (up to 255),
+// which is a root of a scaled root, by 2.5 * 2^-23, so by 2.3e-5 and 7.6e-5.
+constexpr float kNearFirst = 0.5f - 3e-5f, kNearSecond = 0.5f - 9e-5f;
 
 // m and v of one element after the step
 __device__ __forceinline__ void moments(const Args& a, float g, float& m, float& v) {
@@ -188,6 +197,33 @@ __device__ __forceinline__ void exact_codes(const float (&m)[4], const float (&r
   }
 }
 
+// One lane's eight elements (e .. e + 3 and e + 128 .. e + 131) of a full block, every root correctly rounded: read again
+// from memory, which the lane has not written yet, so that the usual path holds less.
+template <typename P, typename G>
+__device__ __noinline__ void exact_lane(const Args& a, const AdamwTensor& t, long long e, float ms, float vs, float mi,
+                                        float vi, float gs) {
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h, e += 128) {
+    float p[4], g[4], m[4], v[4];
+    load4<P>(t.p, e, t.n, true, p);
+    load4<G>(t.g, e, t.n, true, g);
+    uint32_t mw = load_codes(t.m, e, t.n, true), vw = load_codes(t.v, e, t.n, true);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = first_value(mw, j, ms);
+      const float r = root_value(vw, j, vs);
+      v[j] = __fmul_rn(r, r);
+      moments(a, __fmul_rn(g[j], gs), m[j], v[j]);
+      v[j] = __fsqrt_rn(v[j]);
+      p[j] = moved(a, p[j], m[j], v[j]);
+    }
+    exact_codes(m, v, mi, vi, mw, vw);
+    store4<P>(t.p, e, t.n, true, p);
+    store_codes(t.m, e, t.n, true, mw);
+    store_codes(t.v, e, t.n, true, vw);
+  }
+}
+
 // A block of 256 whose elements all exist and whose arrays are aligned, 8-bit moments.
 template <typename P, typename G>
 __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t, long long b, int lane, float gs) {
@@ -203,9 +239,8 @@ __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t,
     vc[h] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + e + 128 * h);
   }
   const float ms = t.m_scale[b], vs = t.v_scale[b];
-  float m[2][4], v[2][4], root[2][4];
+  float m[2][4], root[2][4];
   uint32_t mb = 0, vb = 0;
-  float least = 1.0f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float g[4];
@@ -214,13 +249,12 @@ __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t,
     for (int j = 0; j < 4; ++j) {
       const float c = code_float(mc[h] ^ 0x80808080u, j, 8388736.0f), d = code_float(vc[h], j, 8388608.0f);
       const float r = __fmul_rn(d * d, vs);
+      float v = __fmul_rn(r, r);
       m[h][j] = __fmul_rn(c * fabsf(c), ms);
-      v[h][j] = __fmul_rn(r, r);
-      moments(a, __fmul_rn(g[j], gs), m[h][j], v[h][j]);
+      moments(a, __fmul_rn(g[j], gs), m[h][j], v);
       mb = max(mb, __float_as_uint(m[h][j]) & 0x7FFFFFFFu);
-      vb = max(vb, __float_as_uint(v[h][j]));
-      root[h][j] = root_approx(v[h][j]);
-      least = fminf(least, root[h][j]);
+      vb = max(vb, __float_as_uint(v));
+      root[h][j] = root_approx(v);
     }
   }
   mb = __reduce_max_sync(0xFFFFFFFFu, mb);
@@ -228,7 +262,11 @@ __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t,
   float mi, vi;
   const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi);
   const float vs1 = block_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(vb))), 1.0f / 65025.0f, vi);
-  float far = 0.0f;  // the largest distance of a root from its code
+  const F2 up = f2(kRound, kRound), down = f2(-kRound, -kRound), minus = f2(-1.0f, -1.0f);
+  const F2 rs = f2(a.root_scale, a.root_scale), eps = f2(a.eps, a.eps), decay = f2(a.decay, a.decay);
+  const F2 back = f2(-a.step_size, -a.step_size);
+  float least = kRound + 1.0f;  // the smallest second-moment code: 0 (a vanishing root) goes the exact way
+  float far_m = 0.0f, far_v = 0.0f;  // the largest distances of the roots from their codes
   uint32_t mw[2], vw[2];
   float p[2][4];
 #pragma unroll
@@ -236,42 +274,37 @@ __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t,
     float r[4], q[4];
     Quad<P>::unpack(pv[h], p[h]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = copysignf(root_approx(fabsf(m[h][j]) * mi), m[h][j]), y = root_approx(root[h][j] * vi);
-      r[j] = x + kRound, q[j] = y + kRound;
-      far = fmaxf(far, fmaxf(fabsf(x - (r[j] - kRound)), fabsf(y - (q[j] - kRound))));
-      q[j] = fmaxf(q[j], kRound + 1.0f);  // a vanishing root goes the exact way
-      p[h][j] = p[h][j] * a.decay - a.step_size * __fdividef(m[h][j], root[h][j] * a.root_scale + a.eps);
+    for (int i = 0; i < 4; i += 2) {
+      const F2 s = f2(copysignf(root_approx(fabsf(m[h][i]) * mi), m[h][i]),
+                      copysignf(root_approx(fabsf(m[h][i + 1]) * mi), m[h][i + 1]));
+      const F2 u = f2(root_approx(root[h][i] * vi), root_approx(root[h][i + 1] * vi));
+      const F2 sr = s + up, ur = u + up;
+      float x, y;
+      split(fma2(sr + down, minus, s), x, y);
+      far_m = fmaxf(far_m, fmaxf(fabsf(x), fabsf(y)));
+      split(fma2(ur + down, minus, u), x, y);
+      far_v = fmaxf(far_v, fmaxf(fabsf(x), fabsf(y)));
+      split(sr, r[i], r[i + 1]);
+      split(ur, q[i], q[i + 1]);
+      least = fminf(least, fminf(q[i], q[i + 1]));
+      split(fma2(f2(root[h][i], root[h][i + 1]), rs, eps), x, y);
+      const F2 step = f2(m[h][i], m[h][i + 1]) * f2(reciprocal_approx(x), reciprocal_approx(y));
+      split(fma2(step, back, f2(p[h][i], p[h][i + 1]) * decay), p[h][i], p[h][i + 1]);
     }
     mw[h] = low_bytes(r[0], r[1], r[2], r[3]);
     vw[h] = low_bytes(q[0], q[1], q[2], q[3]);
   }
-  if (!(far < kNearTie) || !(least > 0.0f) || mi == 0.0f || vi == 0.0f) {
-#pragma unroll 1
+  if (!(far_m < kNearFirst) || !(far_v < kNearSecond) || !(least > kRound) || mi == 0.0f || vi == 0.0f) {
+    exact_lane<P, G>(a, t, e, ms, vs, mi, vi, gs);
+  } else {
+#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float exact[4], mh[4], ph[4];
-      const typename Quad<P>::V old = h ? pv[1] : pv[0];
-      Quad<P>::unpack(old, ph);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mh[j] = h ? m[1][j] : m[0][j];
-        exact[j] = __fsqrt_rn(h ? v[1][j] : v[0][j]);
-        ph[j] = moved(a, ph[j], mh[j], exact[j]);
-      }
-      uint32_t x, y;
-      exact_codes(mh, exact, mi, vi, x, y);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (h) p[1][j] = ph[j]; else p[0][j] = ph[j];
-      if (h) mw[1] = x, vw[1] = y; else mw[0] = x, vw[0] = y;
+      *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = Quad<P>::pack(p[h]);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + e + 128 * h) = mw[h];
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + e + 128 * h) = vw[h];
     }
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = Quad<P>::pack(p[h]);
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + e + 128 * h) = mw[h];
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + e + 128 * h) = vw[h];
-  }
+  __syncwarp();  // no lane still wants the old scales
   if (lane == 0) {
     t.m_scale[b] = ms1;
     t.v_scale[b] = vs1;
@@ -377,7 +410,7 @@ __device__ __noinline__ void ragged_block(const Args& a, const AdamwTensor& t, l
 }
 
 template <typename P, typename G, bool k8>
-__global__ void __launch_bounds__(kWarps * 32) adamw_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kWarps * 32, k8 ? (sizeof(P) + sizeof(G) == 4 ? 6 : 5) : 4) adamw_kernel(const __grid_constant__ Args a) {
   // the tensor of this CTA: the last whose first CTA is not past it
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
