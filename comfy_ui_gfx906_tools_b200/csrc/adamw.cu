@@ -262,53 +262,42 @@ __device__ __forceinline__ void full_block8(const Args& a, const AdamwTensor& t,
   float mi, vi;
   const float ms1 = block_scale(mb, 1.0f / 16129.0f, mi);
   const float vs1 = block_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(vb))), 1.0f / 65025.0f, vi);
-  const F2 up = f2(kRound, kRound), down = f2(-kRound, -kRound), minus = f2(-1.0f, -1.0f);
-  const F2 rs = f2(a.root_scale, a.root_scale), eps = f2(a.eps, a.eps), decay = f2(a.decay, a.decay);
-  const F2 back = f2(-a.step_size, -a.step_size);
   float least = kRound + 1.0f;  // the smallest second-moment code: 0 (a vanishing root) goes the exact way
   float far_m = 0.0f, far_v = 0.0f;  // the largest distances of the roots from their codes
   uint32_t mw[2], vw[2];
-  float p[2][4];
+  typename Quad<P>::V out[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float r[4], q[4];
-    Quad<P>::unpack(pv[h], p[h]);
+    float r[4], q[4], p[4];
+    Quad<P>::unpack(pv[h], p);
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      const F2 s = f2(copysignf(root_approx(fabsf(m[h][i]) * mi), m[h][i]),
-                      copysignf(root_approx(fabsf(m[h][i + 1]) * mi), m[h][i + 1]));
-      const F2 u = f2(root_approx(root[h][i] * vi), root_approx(root[h][i + 1] * vi));
-      const F2 sr = s + up, ur = u + up;
-      float x, y;
-      split(fma2(sr + down, minus, s), x, y);
-      far_m = fmaxf(far_m, fmaxf(fabsf(x), fabsf(y)));
-      split(fma2(ur + down, minus, u), x, y);
-      far_v = fmaxf(far_v, fmaxf(fabsf(x), fabsf(y)));
-      split(sr, r[i], r[i + 1]);
-      split(ur, q[i], q[i + 1]);
-      least = fminf(least, fminf(q[i], q[i + 1]));
-      split(fma2(f2(root[h][i], root[h][i + 1]), rs, eps), x, y);
-      const F2 step = f2(m[h][i], m[h][i + 1]) * f2(reciprocal_approx(x), reciprocal_approx(y));
-      split(fma2(step, back, f2(p[h][i], p[h][i + 1]) * decay), p[h][i], p[h][i + 1]);
+    for (int j = 0; j < 4; ++j) {
+      const float x = copysignf(root_approx(fabsf(m[h][j]) * mi), m[h][j]), y = root_approx(root[h][j] * vi);
+      r[j] = x + kRound, q[j] = y + kRound;
+      far_m = fmaxf(far_m, fabsf(x - (r[j] - kRound)));
+      far_v = fmaxf(far_v, fabsf(y - (q[j] - kRound)));
+      least = fminf(least, q[j]);
+      p[j] = p[j] * a.decay - a.step_size * (m[h][j] * reciprocal_approx(root[h][j] * a.root_scale + a.eps));
     }
     mw[h] = low_bytes(r[0], r[1], r[2], r[3]);
     vw[h] = low_bytes(q[0], q[1], q[2], q[3]);
+    out[h] = Quad<P>::pack(p);
   }
-  if (!(far_m < kNearFirst) || !(far_v < kNearSecond) || !(least > kRound) || mi == 0.0f || vi == 0.0f) {
-    exact_lane<P, G>(a, t, e, ms, vs, mi, vi, gs);
-  } else {
+  const bool exactly =
+      !(far_m < kNearFirst) || !(far_v < kNearSecond) || !(least > kRound) || mi == 0.0f || vi == 0.0f;
+  if (!exactly) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = Quad<P>::pack(p[h]);
+      *reinterpret_cast<typename Quad<P>::V*>(static_cast<P*>(t.p) + e + 128 * h) = out[h];
       *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + e + 128 * h) = mw[h];
       *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + e + 128 * h) = vw[h];
     }
   }
-  __syncwarp();  // no lane still wants the old scales
   if (lane == 0) {
     t.m_scale[b] = ms1;
     t.v_scale[b] = vs1;
   }
+  if (exactly) exact_lane<P, G>(a, t, e, ms, vs, mi, vi, gs);
 }
 
 // The same with 32-bit moments.

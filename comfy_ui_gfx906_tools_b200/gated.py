@@ -32,16 +32,18 @@ def _ptr(t: torch.Tensor | None):
 
 def _forward(x, w_gate, w_up, b_gate, b_up, act, keep):
     """(h, the float32 projections that a backward wants: [2, M, F], or None)"""
-    (M, K), N = x.shape, w_gate.shape[0]
-    dev = x.device
-    h = torch.empty((M, N), dtype=x.dtype, device=dev)
-    save = torch.empty((2, M, N), dtype=torch.float32, device=dev) if keep else None
+    (M, K), N, dev = x.shape, w_gate.shape[0], x.device
+    lib = _lib.load()
+    h = x.new_empty((M, N))
+    save = x.new_empty((2, M, N), dtype=torch.float32) if keep else None
     with ops._on(dev):
-        stream, need = ops._stream(dev), _lib.load().gated_linear_workspace_bytes(M, K, N)
-        ws = ops._workspace(dev, stream, need)
-        ops._call_gemm("gated_linear", dev, x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0),
-                       w_up.data_ptr(), w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._dtype_code(x.dtype), act,
-                       h.data_ptr(), _ptr(save), M, K, N, _ptr(ws), ws.numel() if need else 0, stream)
+        stream, need = ops._stream(dev), lib.gated_linear_workspace_bytes(M, K, N)
+        ws = ops._workspace(dev, stream, need) if need else None
+        rc = lib.gated_linear(x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(),
+                              w_up.stride(0), _ptr(b_gate), _ptr(b_up), ops._DTYPE_CODE[x.dtype], act, h.data_ptr(),
+                              _ptr(save), M, K, N, _ptr(ws), ws.numel() if need else 0, stream)
+    if rc:
+        ops._check_gemm("gated_linear", dev, rc)
     return h, save
 
 
@@ -58,17 +60,18 @@ class _GatedLinear(torch.autograd.Function):
     def backward(ctx, dh):
         x, w_gate, w_up, save = ctx.saved_tensors
         (M, K), N = x.shape, w_gate.shape[0]
-        dh = _rows(dh)
+        dh, dev, lib = _rows(dh), x.device, _lib.load()
         shapes = ((M, K), (N, K), (N, K), (N,), (N,))
-        grads = [torch.empty(s, dtype=x.dtype, device=x.device) if need else None
-                 for s, need in zip(shapes, ctx.needs_input_grad)]
-        with ops._on(x.device):
-            ws = torch.empty(_lib.load().gated_linear_backward_workspace_bytes(M, K, N), dtype=torch.uint8,
-                             device=x.device)
-            ops._call_gemm("gated_linear_backward", x.device, dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0),
-                           w_gate.data_ptr(), w_gate.stride(0), w_up.data_ptr(), w_up.stride(0), save.data_ptr(),
-                           ops._dtype_code(x.dtype), ctx.act, *map(_ptr, grads), M, K, N, ws.data_ptr(), ws.numel(),
-                           ops._stream(x.device))
+        grads = [x.new_empty(s) if need else None for s, need in zip(shapes, ctx.needs_input_grad)]
+        with ops._on(dev):
+            ws = x.new_empty(lib.gated_linear_backward_workspace_bytes(M, K, N), dtype=torch.uint8)
+            rc = lib.gated_linear_backward(
+                dh.data_ptr(), dh.stride(0), x.data_ptr(), x.stride(0), w_gate.data_ptr(), w_gate.stride(0),
+                w_up.data_ptr(), w_up.stride(0), save.data_ptr(), ops._DTYPE_CODE[x.dtype], ctx.act,
+                *[g.data_ptr() if g is not None else None for g in grads], M, K, N, ws.data_ptr(), ws.numel(),
+                ops._stream(dev))
+        if rc:
+            ops._check_gemm("gated_linear_backward", dev, rc)
         return (*grads, None)
 
 
@@ -93,22 +96,26 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     N, K = w_gate.shape
     if K % 8 or N % 8 or K == 0 or N == 0:
         raise RuntimeError(f"expected K % 8 == 0 and F % 8 == 0, got K={K} F={N}")
-    for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (b_gate, "b_gate"), (b_up, "b_up")):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise RuntimeError(f"{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
-    for t, name in ((b_gate, "b_gate"), (b_up, "b_up")):
-        if t is not None and tuple(t.shape) != (N,):
+    dt, index = x.dtype, x.get_device()
+    for t, name, shape in ((w_gate, "w_gate", None), (w_up, "w_up", None), (b_gate, "b_gate", (N,)),
+                           (b_up, "b_up", (N,))):
+        if t is None:
+            continue
+        if t.dtype is not dt or t.get_device() != index:
+            raise RuntimeError(f"{name} must be {dt} on {x.device}, got {t.dtype} on {t.device}")
+        if shape and t.shape != shape:
             raise RuntimeError(f"{name} must have {N} elements, got {tuple(t.shape)}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, K)
     if x2.shape[0] > 2 ** 30:
         raise RuntimeError(f"at most 2^30 tokens, got {x2.shape[0]}")
     args = (_rows(x2), _rows(w_gate), _rows(w_up), b_gate.contiguous() if b_gate is not None else None,
             b_up.contiguous() if b_up is not None else None)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
         h = _GatedLinear.apply(*args, ACTIVATIONS[activation])
     else:
         h = _forward(*args, ACTIVATIONS[activation], False)[0]
-    return h if x.dim() == 2 else h.reshape(*x.shape[:-1], N)
+    return h if flat else h.reshape(*x.shape[:-1], N)
 
 
 class GatedMLP(torch.nn.Module):

@@ -38,6 +38,7 @@ _DTYPE_CODE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, tor
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _dtype_code(dt: torch.dtype) -> int:
@@ -59,7 +60,7 @@ _HERE = contextlib.nullcontext()
 def _on(device: torch.device):
     """The context of a call on `device`: nothing to do where it is current, which entering torch.cuda.device would
     find out in some microseconds."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _CURRENT_DEVICE() else torch.cuda.device(device)
 
 
 def _require_cuda(t: torch.Tensor, name: str):
@@ -109,6 +110,14 @@ def device_status(device: torch.device | None = None, clear: bool = False) -> in
             _rearm_workspaces(device)
             torch.cuda.synchronize(device)
     return v
+
+
+def _check_gemm(name: str, device: torch.device, rc: int):
+    """As ``_call_gemm``, on the code that a call returned."""
+    if rc != _lib.GFX_OK:
+        if rc == _lib.GFX_ERR_DEVICE:
+            _rearm_workspaces(device)
+        raise _lib.GfxError(name, rc, _lib.last_error())
 
 
 def _call_gemm(name: str, device: torch.device, *args):

@@ -16,7 +16,8 @@ positive second moment keeps at least the code 1.
 """
 from __future__ import annotations
 
-import ctypes
+import array
+import operator
 
 import torch
 
@@ -30,10 +31,14 @@ def moment_scales(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
+# Whole lists at a time, without a loop of Python's own: a step over many small tensors is bound by this side.
+_DTYPES, _DEVICES = operator.attrgetter("dtype"), torch.Tensor.get_device
+_NUMELS, _CONTIGUOUS, _ADDRESSES = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
 def _lists(params, others):
     """Checks the lists of one step: others is [(name, tensors, dtype or None for the first one's, scales)]; returns
-    (device, elements of each parameter), or None where there is nothing to do. Whole lists are compared at once: a
-    step over many small tensors is bound by this side."""
+    (device, elements of each parameter), or None where there is nothing to do."""
     n = len(params)
     for name, tensors, _, _ in others:
         if len(tensors) != n:
@@ -41,15 +46,16 @@ def _lists(params, others):
     if n == 0:
         return None
     ops._require_cuda(params[0], "params[0]")
-    dev, index, numel = params[0].device, params[0].get_device(), [t.numel() for t in params]
+    dev, index, numel = params[0].device, params[0].get_device(), list(map(_NUMELS, params))
     ops._dtype_code(params[0].dtype)
+    here, yes = [index] * n, [True] * n
     for name, tensors, dtype, scales in (("params", params, None, False), *others):
         dtype = dtype or tensors[0].dtype
-        want = [moment_scales(x) for x in numel] if scales else numel
-        wanted = [(dtype, index, x, True) for x in want]
-        got = [(t.dtype, t.get_device(), t.numel(), t.is_contiguous()) for t in tensors]
-        if got != wanted:
-            i = next(i for i in range(n) if got[i] != wanted[i])
+        want = list(map(moment_scales, numel)) if scales else numel
+        if (list(map(_DTYPES, tensors)) != [dtype] * n or list(map(_DEVICES, tensors)) != here
+                or list(map(_NUMELS, tensors)) != want or list(map(_CONTIGUOUS, tensors)) != yes):
+            i = next(i for i, t in enumerate(tensors) if t.dtype != dtype or t.get_device() != index
+                     or t.numel() != want[i] or not t.is_contiguous())
             t = tensors[i]
             raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {want[i]} elements; got {t.dtype} "
                                f"on {t.device}, {tuple(t.shape)}, strides {t.stride()}")
@@ -67,12 +73,14 @@ def _call(dev, numel, lists, bits, step, lr, betas, eps, weight_decay, grad_scal
     params, grads = lists[:2]
     n = len(params)
     # one host array: a row of pointers for each list, then the element counts
-    rows = [t.data_ptr() for x in lists for t in x]
-    table = (ctypes.c_uint64 * (len(rows) + n))(*rows, *numel)
-    at = ctypes.addressof(table)
-    where = [at + 8 * n * i for i in range(len(lists))]
+    table = array.array("Q")
+    for tensors in lists:
+        table.extend(map(_ADDRESSES, tensors))
+    table.extend(numel)
+    at = table.buffer_info()[0]
+    where = [at + 8 * n * i for i in range(len(lists) + 1)]
     with ops._on(dev):
-        _lib.call("adamw_step", *where[:4], *(where[4:] or (None, None)), at + 8 * len(rows), n,
+        _lib.call("adamw_step", *where[:4], *(where[4:6] if bits == 8 else (None, None)), where[-1], n,
                   ops._dtype_code(params[0].dtype), ops._dtype_code(grads[0].dtype), bits, int(step), float(lr),
                   float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale, ops._stream(dev))
     torch.autograd.graph.increment_version(params)  # autograd sees the kernel's write as any in-place change

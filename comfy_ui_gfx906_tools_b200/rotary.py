@@ -53,20 +53,22 @@ def _like_tokens(x: torch.Tensor) -> torch.Tensor:
     [B, L, H * D] projection lies as that projection does."""
     if x.stride(1) < x.stride(2):
         B, H, L, D = x.shape
-        return torch.empty(B, L, H, D, dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty((B, L, H, D)).transpose(1, 2)
+    return x.new_empty(x.shape)
 
 
 def _forward(q, k, positions, pos_strides, q_scale, k_scale, call):
     B, H, L, D = q.shape
     dev, code, scale_code, kv, tail = q.device, *call
-    q_out = torch.empty((B, H, L, D), dtype=q.dtype, device=dev)
-    k_out = torch.empty((B, kv, L, D), dtype=q.dtype, device=dev) if k is not None else None
+    q_out = q.new_empty((B, H, L, D))
+    k_out = q.new_empty((B, kv, L, D)) if k is not None else None
     keep, (qs, ks, ps, qos, kos) = _strides(q.stride(), _of(k), pos_strides, q_out.stride(), _of(k_out))
     with ops._on(dev):
-        _lib.call("qk_norm_rope", q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(),
-                  _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale), scale_code, q_out.data_ptr(), qos,
-                  _ptr(k_out), kos, B, H, kv, L, D, *tail, ops._stream(dev))
+        rc = _lib.load().qk_norm_rope(
+            q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(), _POSITIONS[positions.dtype], ps, _ptr(q_scale),
+            _ptr(k_scale), scale_code, q_out.data_ptr(), qos, _ptr(k_out), kos, B, H, kv, L, D, *tail, ops._stream(dev))
+    if rc:
+        raise _lib.GfxError("qk_norm_rope", rc, _lib.last_error())
     return q_out, k_out
 
 
@@ -93,11 +95,14 @@ class _QkNormRope(torch.autograd.Function):
         with ops._on(dev):
             ws = None
             if dqs is not None or dks is not None:
-                ws = torch.empty(_lib.load().qk_norm_rope_workspace_bytes(D), dtype=torch.uint8, device=dev)
-            _lib.call("qk_norm_rope_backward", dq_out.data_ptr(), dqo, _ptr(dk_out), dko, q.data_ptr(), qs, _ptr(k),
-                      ks, code, positions.data_ptr(), _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale),
-                      scale_code, dq.data_ptr(), dqi, _ptr(dk), dki, _ptr(dqs), _ptr(dks), B, H, kv, L, D, *tail,
-                      _ptr(ws), ws.numel() if ws is not None else 0, ops._stream(dev))
+                ws = q.new_empty(_lib.load().qk_norm_rope_workspace_bytes(D), dtype=torch.uint8)
+            rc = _lib.load().qk_norm_rope_backward(
+                dq_out.data_ptr(), dqo, _ptr(dk_out), dko, q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(),
+                _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale), scale_code, dq.data_ptr(), dqi, _ptr(dk),
+                dki, _ptr(dqs), _ptr(dks), B, H, kv, L, D, *tail, _ptr(ws), ws.numel() if ws is not None else 0,
+                ops._stream(dev))
+        if rc:
+            raise _lib.GfxError("qk_norm_rope_backward", rc, _lib.last_error())
         return dq, dk, None, dqs, dks, None, None
 
 
@@ -154,6 +159,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         q_scale, k_scale = (s.contiguous() if s is not None else None for s in (q_scale, k_scale))
     args = (_rows(q), _rows(k) if k is not None else None, positions, ps, q_scale, k_scale)
     call = (code, scale_code, kv, (axes, n, float(theta), int(interleaved), float(eps)))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_scale, k_scale)):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (q, k, q_scale, k_scale)]):
         return _QkNormRope.apply(*args[:3], *args[4:], ps, call)
     return _forward(*args, call)
