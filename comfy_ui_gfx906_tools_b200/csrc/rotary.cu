@@ -18,17 +18,17 @@
 // above a float32 result's rounding). Statistics and sums are float32.
 //
 // Memory-bound, but the sines cost more than the rows they turn if every warp
-// computes its own: a block of eight warps first fills a table for its 8 tokens
+// computes its own: a block of four warps first fills a table for its 4 tokens
 // (fewer where the sequence is short), each angle once, and a warp then walks
 // the heads of one token. G = 8, 16 or 32 lanes hold a row, eight elements each
 // (two runs of four where the pairs are split halves), a warp 32 / G heads a
 // step. The rows of three steps (two in the backward, which reads two arrays)
 // are loaded before the first is used, without a branch between the loads.
 // Arithmetic is on pairs of floats, one instruction for two. Measured on B200:
-// forward of 4608 tokens x 48 heads x 128 in bfloat16 (113 MB) 23 us, 4.9 TB/s;
-// 19982 tokens x 40 heads x 64, forward 49 us (205 MB), backward 95 us (307 MB).
+// forward of 4608 tokens x 48 heads x 128 in bfloat16 (113 MB) 21 us, 5.4 TB/s;
+// 19982 tokens x 40 heads x 64, forward 48 us (205 MB), backward 89 us (307 MB).
 // What bounds it is the issue of the 16-bit conversions and the reductions
-// against the latency of the loads, at four blocks an SM (two in the backward).
+// against the latency of the loads, at 32 warps an SM (16 in the backward).
 #include <math.h>
 #include <string.h>
 
@@ -38,7 +38,7 @@
 namespace gfx {
 namespace rotary {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 
 // The eight elements of a lane as they lie in memory: four at p and four at p + gap.
 template <typename T>
@@ -46,7 +46,8 @@ struct Raw {
   uint32_t w[2 * sizeof(T)];
 };
 
-template <typename T, bool kVec>
+// kOnce: a forward's input, which is not wanted in the cache again.
+template <typename T, bool kVec, bool kOnce>
 __device__ __forceinline__ Raw<T> load8(const T* p, int gap) {
   Raw<T> r;
   if constexpr (kVec) {
@@ -54,7 +55,7 @@ __device__ __forceinline__ Raw<T> load8(const T* p, int gap) {
       *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
       *reinterpret_cast<uint4*>(r.w + 4) = *reinterpret_cast<const uint4*>(p + gap);
     } else if (gap == 4) {  // one run of eight
-      *reinterpret_cast<uint4*>(r.w) = *reinterpret_cast<const uint4*>(p);
+      *reinterpret_cast<uint4*>(r.w) = kOnce ? __ldcs(reinterpret_cast<const uint4*>(p)) : *reinterpret_cast<const uint4*>(p);
     } else {
       *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p);
       *reinterpret_cast<uint2*>(r.w + 2) = *reinterpret_cast<const uint2*>(p + gap);
@@ -180,7 +181,7 @@ __device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&c)[2], const F2 (&s)
 // [block][2][D] (q, then k).
 // kVec: every row starts at a multiple of 16 bytes.
 template <typename T, int G, bool kPairs, bool kVec, bool kBackward>
-__global__ void __launch_bounds__(kWarps * 32, kBackward ? 2 : 4) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kRows = 32 / G, kLanePairs = 4 * G;
   constexpr int kAhead = kBackward ? 2 : 3;  // steps whose rows are in flight at once
   __shared__ __align__(16) float scales[2][8 * G];
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 2 : 4) rope_kernel(co
   const int pair = threadIdx.x % kLanePairs;
   const double freq = pair < half ? a.freq[pair] : 0.0;
   const long long axis_at = pair < half ? a.axis[pair] * a.pos_stride[2] : 0;
-  const uint32_t tokens = a.tokens, group = a.group;  // tokens a block holds at once: 1, 2, 4 or 8
+  const uint32_t tokens = a.tokens, group = a.group;  // tokens a block holds at once: 1, 2 or 4
   const int slot = warp % group;                      // this warp's token of them
   const int part = warp / group + (int)blockIdx.y * (kWarps / group);
 
@@ -266,8 +267,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 2 : 4) rope_kernel(co
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
           const bool row = i0 + q < count;
-          in[q] = load8<T, kVec>(row ? src : in0, row ? gap : 4);
-          if (kBackward && norm) xs[q] = load8<T, kVec>(row ? org : org0, row ? gap : 4);
+          in[q] = load8<T, kVec, !kBackward>(row ? src : in0, row ? gap : 4);
+          if (kBackward && norm) xs[q] = load8<T, kVec, !kBackward>(row ? org : org0, row ? gap : 4);
           src += src_step;
           if (kBackward) org += org_step;
         }
@@ -416,14 +417,14 @@ void rope_frequencies(RopeArgs* a, const int* axes_dims, int n_axes, double thet
   a->axes = n_axes;
 }
 
-// A block's eight warps hold 8 tokens, or fewer with several warps a token where that leaves less than three blocks an
-// SM (at six, 993 tokens of 16 heads took 9 us instead of 5); a lone token's heads are spread over blocks too, down to one step a warp. A backward that sums scale
+// A block's four warps hold 4 tokens, or fewer with several warps a token where that leaves less than six blocks an SM
+// (at twelve, 4608 tokens of 48 heads took 23 us instead of 21); a lone token's heads are spread over blocks too, down to one step a warp. A backward that sums scale
 // gradients keeps to a fixed number of blocks, which walk the tokens.
 static dim3 plan(RopeArgs* a, int rows, int sms) {
   const long long tokens = (long long)a->B * a->L;
   const int steps = (a->heads[0] + rows - 1) / rows + (a->heads[1] + rows - 1) / rows;
   int group = rotary::kWarps;
-  while (group > 1 && tokens / group < 3ll * sms) group /= 2;
+  while (group > 1 && tokens / group < 6ll * sms) group /= 2;
   const int warps = rotary::kWarps / group;  // of a token, in one block
   int spread = 1;
   while (group == 1 && spread * warps < steps && tokens * spread < sms) ++spread;
