@@ -411,6 +411,8 @@ __global__ void __launch_bounds__(kWarps * 32, k8 ? (sizeof(P) + sizeof(G) == 4 
   const long long b0 = (long long)((int)blockIdx.x - t.first_cta) * a.blocks_per_cta;
   const long long b1 = b0 + a.blocks_per_cta < blocks ? b0 + a.blocks_per_cta : blocks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   const float gs = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
   for (long long b = b0 + warp; b < b1; b += kWarps) {
     if (t.aligned != 0 && (b + 1) * kBlock <= n) {
@@ -429,6 +431,8 @@ __global__ void __launch_bounds__(kWarps * 32) moment_values_kernel(const void* 
   const int lane = threadIdx.x & 31;
   const long long blocks = (n + kBlock - 1) / kBlock;
   constexpr int kAhead = 4;  // blocks whose codes are in flight at once
+  pdl_trigger();
+  pdl_wait();
   const long long stride = (long long)gridDim.x * kWarps;
   for (long long b = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); b < blocks; b += kAhead * stride) {
     uint32_t w[kAhead][2];
@@ -460,9 +464,9 @@ __global__ void __launch_bounds__(kWarps * 32) moment_values_kernel(const void* 
 template <typename P, typename G>
 static int launch_adamw_t(const adamw::Args& a, bool bits8, int ctas, cudaStream_t st) {
   if (bits8)
-    adamw::adamw_kernel<P, G, true><<<ctas, adamw::kWarps * 32, 0, st>>>(a);
+    launch_overlapped(adamw::adamw_kernel<P, G, true>, dim3(ctas), adamw::kWarps * 32, st, a);
   else
-    adamw::adamw_kernel<P, G, false><<<ctas, adamw::kWarps * 32, 0, st>>>(a);
+    launch_overlapped(adamw::adamw_kernel<P, G, false>, dim3(ctas), adamw::kWarps * 32, st, a);
   return check_launch("adamw_kernel");
 }
 
@@ -516,9 +520,9 @@ int launch_moment_values(const void* codes, const float* scale, float* out, long
   const long long need = ((n + adamw::kBlock - 1) / adamw::kBlock + adamw::kWarps - 1) / adamw::kWarps;
   const int ctas = (int)(need < (long long)sms * 8 ? need : (long long)sms * 8);
   if (second)
-    adamw::moment_values_kernel<true><<<ctas, adamw::kWarps * 32, 0, st>>>(codes, scale, out, n, vec);
+    launch_overlapped(adamw::moment_values_kernel<true>, dim3(ctas), adamw::kWarps * 32, st, codes, scale, out, n, vec);
   else
-    adamw::moment_values_kernel<false><<<ctas, adamw::kWarps * 32, 0, st>>>(codes, scale, out, n, vec);
+    launch_overlapped(adamw::moment_values_kernel<false>, dim3(ctas), adamw::kWarps * 32, st, codes, scale, out, n, vec);
   return check_launch("moment_values_kernel");
 }
 

@@ -403,6 +403,22 @@ unsigned failure_epoch(int dev);
 // counters, if any) are re-zeroed on `stream` before returning.
 int check_device_health(const char* fn, int dev, void* workspace, size_t counter_bytes, cudaStream_t stream);
 
+// A launch that may start while the stream's previous kernel ends (programmatic dependent launch): the kernel calls
+// pdl_wait() before it touches global memory.
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Argument checks shared by the GEMM entry points (messages name `fn`).
 int check_gemm_common(const char* fn, const void* x, int x_dtype, const void* w, const void* ws, int scale_dtype,
                       void* y, int out_dtype, int M, int N, int K, int splits);

@@ -26,6 +26,8 @@ constexpr int kRowsPerBlock = 64;
 template <typename T, int kAct>
 __global__ void __launch_bounds__(256) gate_grad_kernel(const T* dh, long long ldh, const float* save, T* dgu,
                                                         float* partial, int* counters, int M, int F) {
+  pdl_trigger();
+  pdl_wait();
   // the products that follow want their counters at zero
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int i = threadIdx.x; i < (int)(kGatedCounterBytes / sizeof(int)); i += 256) counters[i] = 0;
@@ -76,10 +78,13 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const T* dh, long long l
 template <typename T>
 __global__ void __launch_bounds__(256) bias_grad_kernel(const float* partial, int blocks, int F, T* dbg, T* dbu) {
   const int c = blockIdx.x * 256 + threadIdx.x;
+  pdl_trigger();
+  pdl_wait();
   if (c >= 2 * F) return;
   T* out = c < F ? dbg : dbu;
   if (out == nullptr) return;
   float v = 0.0f;
+#pragma unroll 8
   for (int b = 0; b < blocks; ++b) v += partial[(long long)b * 2 * F + c];
   out[c < F ? c : c - F] = from_f32<T>(v);
 }
@@ -122,7 +127,8 @@ static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long lo
   const bool bias = d.b_gate || d.b_up;
   const dim3 grid(blocks, (a.F + 127) / 128);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, st>>>((const T*)dh, ldh, save, dgu, bias ? partial : nullptr, static_cast<int*>(workspace), a.M, a.F);
+    launch_overlapped(kern, grid, 256, st, (const T*)dh, ldh, save, dgu, bias ? partial : nullptr,
+                      static_cast<int*>(workspace), a.M, a.F);
   };
   if (act == gated::kSilu)
     go(gated::gate_grad_kernel<T, gated::kSilu>);
@@ -133,7 +139,8 @@ static int gated_backward_t(const GatedArgs& a, int act, const void* dh, long lo
   int rc = check_launch("gate_grad_kernel");
   if (rc) return rc;
   if (bias) {
-    gated::bias_grad_kernel<T><<<(2 * a.F + 255) / 256, 256, 0, st>>>(partial, blocks, a.F, (T*)d.b_gate, (T*)d.b_up);
+    launch_overlapped(gated::bias_grad_kernel<T>, dim3((2 * a.F + 255) / 256), 256, st, partial, blocks, a.F,
+                      (T*)d.b_gate, (T*)d.b_up);
     if ((rc = check_launch("bias_grad_kernel"))) return rc;
   }
   constexpr int kDtype = std::is_same<T, __half>::value ? GFX_DTYPE_F16 : GFX_DTYPE_BF16;

@@ -233,12 +233,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
   cluster_sync_all();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_base;
+  pdl_trigger();
 
   bool ok = true;
   if (warp == kLoadWarp) {
     if (lane == 0) {
       tma_prefetch_desc(&a.a0);
       tma_prefetch_desc(&a.b0);
+      pdl_wait();
       uint32_t it = 0;
       for (int u = pair; u < units && ok; u += pairs) {
         const Unit w = unit_at(a, u, stages);
@@ -369,6 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
     if (!mbar_wait(drain, 0, kDevErrMmaBarrierTimeout)) ok = false;
   } else {
     const int quadrant = warp & 3, side = warp >> 2;  // 32 TMEM lanes; which half of the columns
+    pdl_wait();
     int n = 0;
     for (int u = pair; u < units && ok; u += pairs, ++n) {
       const Unit w = unit_at(a, u, stages);
@@ -498,14 +501,16 @@ static int launch_pair_blocks(TcArgs& a, cudaStream_t st, int sms) {
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return set_error(GFX_ERR_CUDA, "gated pair_kernel: no current device");
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (pairs_at_once[dev] == 0) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     int n = 0;

@@ -193,6 +193,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
   const bool apart = !kPairs && 8 * sub < 2 * half;
   const int e0 = apart ? 4 * sub : 8 * sub, gap = kPairs ? 4 : (apart ? half : 4);
   const bool live = 8 * sub < D;
+  pdl_trigger();
+  pdl_wait();
   for (int i = threadIdx.x; i < 16 * G; i += kWarps * 32) {
     const int w = i / (8 * G), e = i % (8 * G);
     scales[w][e] = a.t[w].scale != nullptr && e < D ? scale_at(a.t[w].scale, a.scale_dtype, e) : 0.0f;
@@ -371,6 +373,8 @@ __global__ void __launch_bounds__(1024) scale_grad_kernel(const float* partial, 
   __shared__ float s[128][9];
   const int x = threadIdx.x & 7, y = threadIdx.x >> 3, e = blockIdx.x * 8 + x, t = blockIdx.y;
   const float* from = partial + (long long)t * D + e;
+  pdl_trigger();
+  pdl_wait();
   float v = 0.0f;
 #pragma unroll 8
   for (int b = y; b < blocks; b += 128) v += from[(long long)b * 2 * D];
@@ -440,9 +444,9 @@ static int lanes_per_row(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : 32); }
 template <typename T, int G, bool kPairs, bool kVec>
 static int launch_t(const RopeArgs& a, bool backward, dim3 blocks, cudaStream_t st) {
   if (backward)
-    rotary::rope_kernel<T, G, kPairs, kVec, true><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
+    launch_overlapped(rotary::rope_kernel<T, G, kPairs, kVec, true>, blocks, rotary::kWarps * 32, st, a);
   else
-    rotary::rope_kernel<T, G, kPairs, kVec, false><<<blocks, rotary::kWarps * 32, 0, st>>>(a);
+    launch_overlapped(rotary::rope_kernel<T, G, kPairs, kVec, false>, blocks, rotary::kWarps * 32, st, a);
   return check_launch("rope_kernel");
 }
 
@@ -472,8 +476,8 @@ int launch_rope(RopeArgs& a, int dtype, bool pairs, bool backward, void* dq_scal
   else
     rc = launch_g<__nv_bfloat16>(a, pairs, backward, blocks, st);
   if (rc || !backward || a.partial == nullptr) return rc;
-  rotary::scale_grad_kernel<<<dim3(a.D / 8, 2), 1024, 0, st>>>(a.partial, (int)(blocks.x * blocks.y), a.D, dq_scale,
-                                                               dk_scale, a.scale_dtype);
+  launch_overlapped(rotary::scale_grad_kernel, dim3(a.D / 8, 2), 1024, st, a.partial, (int)(blocks.x * blocks.y), a.D,
+                    dq_scale, dk_scale, a.scale_dtype);
   return check_launch("scale_grad_kernel");
 }
 
