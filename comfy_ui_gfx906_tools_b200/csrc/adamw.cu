@@ -20,15 +20,18 @@
 // number, so it is not lost). A lane holds elements 4 l .. 4 l + 3 of each
 // 128-element half, so every access of the warp is one contiguous run.
 //
-// With 8-bit moments the arithmetic would take longer than the memory if every
-// root were correctly rounded (100 instructions an element, 758 us for 151 M
-// bfloat16 elements against 232 us of memory). The full blocks' path takes the
-// hardware's approximate roots, off by 2^-23, and decides a code by them unless
-// the root lies so near the middle between two codes that this error could
-// matter; a lane that sees such an element (one in five thousand), or a
-// vanishing root, does its eight elements again exactly. Codes are turned into
-// floats and back by adding 2^23 and 1.5 * 2^23, not by the quarter-rate
-// conversions.
+// Measured on B200, 151 M bfloat16 elements: 32-bit moments 492 us, 6.7 TB/s,
+// the memory's rate. With 8-bit moments (1.52 GB, 232 us of memory) the
+// arithmetic takes longer than the memory: 441 us, bound by the issue of 74
+// instructions an element. With every root correctly rounded it was 100
+// instructions and 758 us, so the full blocks' path takes the hardware's
+// approximate roots, off by 2^-23, and decides a code by them unless the root
+// lies so near the middle between two codes that this error could matter; a
+// lane that sees such an element (one in five thousand), or a vanishing root,
+// does its eight elements again exactly. Codes are turned into floats and back
+// by adding 2^23 and 1.5 * 2^23, not by the quarter-rate conversions. Packed
+// pairs of floats are not used here: the compiler fuses a packed product and
+// sum, and the moments' definition rounds both.
 #include "common.cuh"
 #include "kernels.h"
 

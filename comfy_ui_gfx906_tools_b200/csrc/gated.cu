@@ -21,6 +21,8 @@ namespace gated {
 // ---------------------------------------------------------------------------
 // dg, du (one row of dgu [M, 2F]: dg then du) and, per block of rows, their column sums
 // ---------------------------------------------------------------------------
+// Memory-bound: float32 g and u and 16-bit dh read, dg and du written, 14 bytes an element; 128 us for 4608 x 12288
+// (792 MB), 6.2 TB/s.
 constexpr int kRowsPerBlock = 64;
 
 template <typename T, int kAct>
