@@ -101,6 +101,8 @@ size_t gated_forward_workspace(int M, int K, int F, int sms) {
 
 int launch_gated_forward(const GatedArgs& a, int dtype, int act, void* h, float* save, void* workspace,
                          cudaStream_t st, int sms) {
+  // Up to 128 tokens (the few-token form's TMEM holds no more) that form is the faster one everywhere measured: 128
+  // tokens at 3072 x 12288 take 43 us there and 45 in 256-row tiles, at 2048 x 5632 20 and 21, one token 29 and 54.
   if (a.M <= kGatedFewTokens) return launch_gated_forward_few(a, dtype, act, h, save, st, sms);
   return launch_gated_forward_tc(a, dtype, act, h, save, workspace, st, sms);
 }

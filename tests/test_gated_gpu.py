@@ -121,6 +121,21 @@ def test_gradients(cuda, shape, act, bias, dtype):
         _near(t, *w, name)
 
 
+@pytest.mark.parametrize("shape", [(3, 64, 20000), (2600, 136, 6008), (1300, 1032, 4808), (5000, 72, 520)], ids=str)
+def test_many_tiles(cuda, shape):
+    """Several waves of tiles: the few-token kernel with more tiles than SMs, the products with one and two row blocks a
+    tile, a contraction shorter than the pipeline, a last wave that is cut."""
+    M, K, F = shape
+    leaves, dh = _inputs(cuda, M, K, F, torch.bfloat16, True, 21)
+    h = gated.gated_linear(*leaves)
+    want, far, grads = _reference(*leaves, "silu", dh)
+    _close(h, want, far)
+    with torch.no_grad():
+        assert torch.equal(gated.gated_linear(*leaves), h)
+    for name, t, w in zip(("x", "w_gate", "w_up", "b_gate", "b_up"), torch.autograd.grad(h, leaves, dh), grads):
+        _near(t, *w, name)
+
+
 def test_gradient_against_differences(cuda):
     """Along the gradient's own signs with an exact step, in float16: the slope is the sum of the gradient's sizes.
     A step of 2^-9 bends the value by parts in a thousand; h's rounding (2^-12 of each of 64 x 256 elements, random

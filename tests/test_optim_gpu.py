@@ -80,6 +80,28 @@ def test_many_tensors_take_several_launches(cuda):
         _close(c, wv, fv)
 
 
+def test_large_tensor(cuda):
+    """Enough elements that a warp takes several blocks, in both forms."""
+    size = (4_000_003,)
+    p, g, m, v = _tensors(cuda, [size], torch.bfloat16, torch.bfloat16, 6)
+    want = _formula(p[0], g[0], m[0], v[0], step=9, **HYPER)
+    optim.adamw_step(p, g, m, v, step=9, **HYPER)
+    for got, w, far in zip((p[0], m[0], v[0]), want[:3], want[3:]):
+        _close(got, w, far)
+    p, g, mc, ms, vc, vs, n = _eight(cuda, size, torch.bfloat16, torch.bfloat16, 7)
+    m0, r0 = _value(mc.cpu(), ms.cpu()), _value(vc.cpu(), vs.cpu())
+    want = _formula(p.cpu(), g.cpu(), m0, r0 * r0, step=9, **HYPER)
+    gf, (b1, b2) = g.cpu().float(), HYPER["betas"]
+    f = lambda x: torch.tensor(x, dtype=torch.float32)  # noqa: E731
+    m1 = m0 * f(b1) + gf * f(1 - b1)
+    v1 = r0 * r0 * f(b2) + gf * gf * f(1 - b2)
+    optim.adamw_step_8bit([p], [g], [mc], [ms], [vc], [vs], step=9, **HYPER)
+    _close(p.cpu(), want[0], want[3])
+    for code, scale, x, top in ((mc, ms, m1, 127), (vc, vs, _sqrt(v1), 255)):
+        wc, ws = _encode(x, top)
+        assert torch.equal(code.cpu().float(), wc) and torch.equal(scale.cpu(), ws)
+
+
 def test_neighbours_of_a_tensor_are_not_written(cuda):
     """Views of one buffer with a gap between them: the gaps keep their values."""
     buf = [torch.full((1000,), 7.0, device=cuda) for _ in range(4)]

@@ -104,6 +104,8 @@ CASES = [
     (1, 1, 1, 1, 8, (2,), True, (True, True), "int", "plain"),
     (1, 7, 2, 300, 80, (16, 32, 32), False, (True, True), "float", "odd"),
     (2, 2, 1, 9, 200, (30, 70), True, (True, True), "int", "plain"),
+    (1, 3, 1, 6001, 64, (16, 24, 24), False, (True, True), "int", "packed"),  # more tokens than a backward's blocks hold
+    (2, 5, 2, 1003, 128, (16, 56, 56), True, (True, True), "large", "odd"),
 ]
 
 
@@ -128,6 +130,32 @@ def test_forward_and_gradient(cuda, case, dtype):
         _close(grads[id(x)], dx, far_dx)
         if w is not None:
             _close(grads[id(w)], dw, far_dw)
+
+
+@pytest.mark.parametrize("dtype,scale_dtype", [(torch.float32, torch.bfloat16), (torch.float16, torch.float32),
+                                               (torch.bfloat16, torch.float16)])
+def test_scales_of_another_type_and_heads_in_one(cuda, dtype, scale_dtype):
+    """A scale of its own type; k as one head expanded over four: its gradient is their sum, made by autograd from the
+    kernel's gradient of each."""
+    q, _ = _inputs(cuda, 2, 3, 1, 21, 64, dtype, "plain", 30)
+    g = torch.Generator().manual_seed(31)
+    one = torch.randn(2, 1, 21, 64, generator=g).to(dtype).to(cuda).requires_grad_(True)
+    w = (1 + 0.2 * torch.randn(64, generator=g)).to(scale_dtype).to(cuda).requires_grad_(True)
+    pos = _positions(2, 21, 3, "int", 30)
+    dq, dk = (torch.randn(2, n, 21, 64, generator=g).to(dtype).to(cuda) for n in (3, 4))
+    yq, yk = rotary.qk_norm_rope(q, one.expand(2, 4, 21, 64), pos.to(cuda), (16, 24, 24), 10000.0, w, w)
+    gq, gk, gw = torch.autograd.grad([yq, yk], [q, one, w], [dq, dk])
+    angle = _angles(pos.expand(2, 21, 3), (16, 24, 24), 10000.0)
+    want, far, dx, far_dx, dw, far_dw = _reference(q, w, angle, True, dq)
+    _close(yq, want, far)
+    _close(gq, dx, far_dx)
+    want, far, dx, far_dx, dw2, far_dw2 = _reference(one.expand(2, 4, 21, 64), w, angle, True, dk)
+    _close(yk, want, far)
+    # autograd adds four gradients of the type, rounding each of three sums
+    total = dx.sum(1, keepdim=True)
+    _close(gk, total, far_dx.sum(1, keepdim=True) + 4 * HALF_STEP[dtype] * dx.abs().sum(1, keepdim=True))
+    # the two scales' gradients, of the scale's type each, added in it
+    _close(gw, dw + dw2, far_dw + far_dw2 + HALF_STEP[scale_dtype] * (dw + dw2).abs() * 1.01)
 
 
 def test_gradient_against_differences(cuda):
