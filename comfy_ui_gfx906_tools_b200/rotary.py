@@ -9,6 +9,7 @@ and writes the [B, H, L, D] layout that attention takes.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 
@@ -27,8 +28,10 @@ def _axes(dims: tuple):
 
 def _strides(*lists):
     """One int64 array of three strides for each list, and the address of each."""
-    flat = (ctypes.c_int64 * (3 * len(lists)))(*[s for x in lists for s in x[:3]])
-    at = ctypes.addressof(flat)
+    flat = array.array("q")
+    for x in lists:
+        flat.extend(x[:3])
+    at = flat.buffer_info()[0]
     return flat, range(at, at + 24 * len(lists), 24)
 
 
@@ -59,14 +62,19 @@ def _like_tokens(x: torch.Tensor) -> torch.Tensor:
 
 def _forward(q, k, positions, pos_strides, q_scale, k_scale, call):
     B, H, L, D = q.shape
-    dev, code, scale_code, kv, tail = q.device, *call
+    dev = q.device
+    code, scale_code, pos_code, kv, tail = call
     q_out = q.new_empty((B, H, L, D))
-    k_out = q.new_empty((B, kv, L, D)) if k is not None else None
-    keep, (qs, ks, ps, qos, kos) = _strides(q.stride(), _of(k), pos_strides, q_out.stride(), _of(k_out))
+    q_strides, k_strides = (H * L * D, L * D, D), (kv * L * D, L * D, D)
+    k_at = k_out_at = k_out = None
+    if k is not None:
+        k_out = q.new_empty((B, kv, L, D))
+        k_at, k_out_at = k.data_ptr(), k_out.data_ptr()
+    keep, (qs, ks, ps, qos, kos) = _strides(q.stride(), _of(k), pos_strides, q_strides, k_strides)
     with ops._on(dev):
-        rc = _lib.load().qk_norm_rope(
-            q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(), _POSITIONS[positions.dtype], ps, _ptr(q_scale),
-            _ptr(k_scale), scale_code, q_out.data_ptr(), qos, _ptr(k_out), kos, B, H, kv, L, D, *tail, ops._stream(dev))
+        rc = _lib.load().qk_norm_rope(q.data_ptr(), qs, k_at, ks, code, positions.data_ptr(), pos_code, ps,
+                                      _ptr(q_scale), _ptr(k_scale), scale_code, q_out.data_ptr(), qos, k_out_at, kos,
+                                      B, H, kv, L, D, *tail, ops._stream(dev))
     if rc:
         raise _lib.GfxError("qk_norm_rope", rc, _lib.last_error())
     return q_out, k_out
@@ -84,7 +92,7 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, positions, q_scale, k_scale = ctx.saved_tensors
         B, H, L, D = q.shape
-        dev, code, scale_code, kv, tail = q.device, *ctx.call
+        dev, code, scale_code, pos_code, kv, tail = q.device, *ctx.call
         dq_out = _rows(dq_out)
         dk_out = _rows(dk_out) if k is not None else None
         dq, dk = _like_tokens(q), _like_tokens(k) if k is not None else None
@@ -98,7 +106,7 @@ class _QkNormRope(torch.autograd.Function):
                 ws = q.new_empty(_lib.load().qk_norm_rope_workspace_bytes(D), dtype=torch.uint8)
             rc = _lib.load().qk_norm_rope_backward(
                 dq_out.data_ptr(), dqo, _ptr(dk_out), dko, q.data_ptr(), qs, _ptr(k), ks, code, positions.data_ptr(),
-                _POSITIONS[positions.dtype], ps, _ptr(q_scale), _ptr(k_scale), scale_code, dq.data_ptr(), dqi, _ptr(dk),
+                pos_code, ps, _ptr(q_scale), _ptr(k_scale), scale_code, dq.data_ptr(), dqi, _ptr(dk),
                 dki, _ptr(dqs), _ptr(dks), B, H, kv, L, D, *tail, _ptr(ws), ws.numel() if ws is not None else 0,
                 ops._stream(dev))
         if rc:
@@ -122,43 +130,49 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     i + sum(axes_dims) / 2. Pair j of an axis of d elements turns by
     position * theta^(-2j/d). q_scale / k_scale [D]: the norm's scale (None:
     that tensor is not normalised). Differentiable in q, k and the scales."""
-    ops._require_cuda(q, "q")
-    code = ops._dtype_code(q.dtype)
-    if q.dim() != 4:
-        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(q.shape)}")
-    dev, (B, _, L, D) = q.device, q.shape
+    index, dt, shape = q.get_device(), q.dtype, q.shape
+    if index < 0:
+        ops._require_cuda(q, "q")
+    code = ops._dtype_code(dt)
+    if len(shape) != 4:
+        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(shape)}")
+    B, _, L, D = shape
     kv = 0
     if k is not None:
-        if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:] or k.dtype != q.dtype or k.device != dev:
-            raise RuntimeError(f"k must be {q.dtype} [{B}, KVH, {L}, {D}] on {dev}, got {k.dtype} {tuple(k.shape)} on "
+        other = k.shape
+        if (len(other) != 4 or other[0] != B or other[2] != L or other[3] != D or k.dtype is not dt
+                or k.get_device() != index):
+            raise RuntimeError(f"k must be {dt} [{B}, KVH, {L}, {D}] on {q.device}, got {k.dtype} {tuple(other)} on "
                                f"{k.device}")
-        kv = k.shape[1]
+        kv = other[1]
     elif k_scale is not None:
         raise RuntimeError("k_scale without k")
     axes = _axes(tuple(axes_dims))
-    n = len(axes)
-    if positions.dtype not in _POSITIONS:
+    n, pos_code = len(axes), _POSITIONS.get(positions.dtype)
+    if pos_code is None:
         raise RuntimeError(f"positions must be float32, int32 or int64, got {positions.dtype}")
-    if positions.device != dev:
-        raise RuntimeError(f"positions must be on {dev}, got {positions.device}")
-    shape, ps = tuple(positions.shape), positions.stride()
-    if shape == (L, n):
+    if positions.get_device() != index:
+        raise RuntimeError(f"positions must be on {q.device}, got {positions.device}")
+    given, ps = positions.shape, positions.stride()
+    if given == (L, n):
         ps = (0, *ps)
-    elif shape == (1, L, n):
+    elif given == (1, L, n):
         ps = (0, ps[1], ps[2])
-    elif shape != (B, L, n):
-        raise RuntimeError(f"positions must be [{L}, {n}] or [{B}, {L}, {n}], got {shape}")
+    elif given != (B, L, n):
+        raise RuntimeError(f"positions must be [{L}, {n}] or [{B}, {L}, {n}], got {tuple(given)}")
     scale_code = code
     first = q_scale if q_scale is not None else k_scale
     if first is not None:
+        scale_type = first.dtype
         for s in (q_scale, k_scale):
-            if s is not None and (s.numel() != D or s.dtype != first.dtype or s.device != dev):
-                raise RuntimeError(f"scales must be [{D}] of one dtype on {dev}, got {s.dtype} {tuple(s.shape)} on "
+            if s is not None and (s.numel() != D or s.dtype is not scale_type or s.get_device() != index):
+                raise RuntimeError(f"scales must be [{D}] of one dtype on {q.device}, got {s.dtype} {tuple(s.shape)} on "
                                    f"{s.device}")
-        scale_code = ops._dtype_code(first.dtype)
+        scale_code = ops._dtype_code(scale_type)
         q_scale, k_scale = (s.contiguous() if s is not None else None for s in (q_scale, k_scale))
-    args = (_rows(q), _rows(k) if k is not None else None, positions, ps, q_scale, k_scale)
-    call = (code, scale_code, kv, (axes, n, float(theta), int(interleaved), float(eps)))
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (q, k, q_scale, k_scale)]):
-        return _QkNormRope.apply(*args[:3], *args[4:], ps, call)
-    return _forward(*args, call)
+    q, k = _rows(q), _rows(k) if k is not None else None
+    call = (code, scale_code, pos_code, kv, (axes, n, float(theta), int(interleaved), float(eps)))
+    if torch.is_grad_enabled() and (q.requires_grad or any([t is not None and t.requires_grad
+                                                            for t in (k, q_scale, k_scale)])):
+        return _QkNormRope.apply(q, k, positions, q_scale, k_scale, ps, call)
+    return _forward(q, k, positions, ps, q_scale, k_scale, call)
