@@ -79,3 +79,39 @@ def test_runs_repeat(cuda):
     b = train_dit.train(train_dit.GatedDiTConfig(depth=1), 5, state_bits=8)
     assert len(a) == 5 and a[0] == b[0]  # the first forward is the same bit for bit
     assert all(abs(x - y) <= 1e-2 * abs(x) for x, y in zip(a, b))
+
+
+def test_operators_in_a_cuda_graph(cuda):
+    """Forward calls and an AdamW step captured once and replayed on new contents of the same tensors."""
+    from comfy_ui_gfx906_tools_b200 import gated, optim, rotary
+    g = torch.Generator().manual_seed(5)
+    make = lambda *s: torch.randn(*s, generator=g).bfloat16().to(cuda)  # noqa: E731
+    few, many, w = make(40, 264), make(700, 264), make(2 * 1032, 264) / 16
+    q, ids = make(1, 4, 33, 64), train_dit.grid_ids(3, 11, cuda)
+    p, grad = torch.ones(5000, device=cuda), torch.randn(5000, generator=g).to(cuda)
+    m, v = torch.zeros(5000, device=cuda), torch.zeros(5000, device=cuda)
+
+    def once():
+        outs = [gated.gated_linear(x, w[:1032], w[1032:]) for x in (few, many)]
+        outs.append(rotary.qk_norm_rope(q, None, ids, (16, 24, 24), q_scale=q[0, 0, 0])[0])
+        optim.adamw_step([p], [grad], [m], [v], step=3, lr=1e-2)
+        return outs
+
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        once()  # workspaces are made outside the capture
+    torch.cuda.current_stream(cuda).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = once()
+    for t in (few, many, q):
+        t.copy_(make(*t.shape))
+    for t in (p, m, v):
+        t.fill_(0.5)
+    graph.replay()
+    got = [t.clone() for t in outs + [p, m, v]]
+    for t in (p, m, v):
+        t.fill_(0.5)
+    want = once() + [p, m, v]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
