@@ -311,7 +311,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
           F2 f[4];
           unpack<T, kPairs>(in[q], f);
           if (norm) {
-            const float r = rsqrtf(ss[q] * a.inv_dim + a.eps);
+            float r = rsqrtf(ss[q] * a.inv_dim + a.eps);
+            // a lane without a row has ss = 0: with eps = 0 its r would be infinite, and 0 * r in dw a NaN
+            if (kBackward && i0 + q >= count) r = 0.0f;
             const F2 rr = f2(r, r);
             if constexpr (!kBackward) {
 #pragma unroll
