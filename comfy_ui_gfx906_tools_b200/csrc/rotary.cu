@@ -166,21 +166,32 @@ __device__ __forceinline__ float scale_at(const void* w, int dtype, int i) {
   return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-// Pairs (f[0..1], f[2..3]) turned by angles of cosine c and sine s; ns = -s.
-__device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&c)[2], const F2 (&s)[2], const F2 (&ns)[2]) {
+// Pairs (f[0..1], f[2..3]) turned by angles of cosine c and sine s; ns = -s. Unless kWhole, only the first n of the four
+// are turned: a pair that passes through keeps its values, which a turn by the angle 0 would not do (an infinity times
+// the sine 0 is a NaN in the pair's other value).
+template <bool kWhole>
+__device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&c)[2], const F2 (&s)[2], const F2 (&ns)[2], int n) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const F2 x = f[i], y = f[2 + i];
     f[i] = fma2(x, c[i], y * ns[i]);
     f[2 + i] = fma2(x, s[i], y * c[i]);
+    if constexpr (!kWhole) {
+      float x0, x1, y0, y1, a, b;
+      split(x, x0, x1), split(y, y0, y1);
+      split(f[i], a, b);
+      f[i] = f2(n > 2 * i ? a : x0, n > 2 * i + 1 ? b : x1);
+      split(f[2 + i], a, b);
+      f[2 + i] = f2(n > 2 * i ? a : y0, n > 2 * i + 1 ? b : y1);
+    }
   }
 }
 
 // kBackward: in is dy, x the forward's input (read where the tensor has a
 // scale), out is dx, and each block leaves its sums of dz xh in partial
 // [block][2][D] (q, then k).
-// kVec: every row starts at a multiple of 16 bytes.
-template <typename T, int G, bool kPairs, bool kVec, bool kBackward>
+// kVec: every row starts at a multiple of 16 bytes. kWhole: no pair passes through.
+template <typename T, int G, bool kPairs, bool kVec, bool kBackward, bool kWhole>
 __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kRows = 32 / G, kLanePairs = 4 * G;
   constexpr int kAhead = kBackward ? 2 : 3;  // steps whose rows are in flight at once
@@ -193,6 +204,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
   const bool apart = !kPairs && 8 * sub < 2 * half;
   const int e0 = apart ? 4 * sub : 8 * sub, gap = kPairs ? 4 : (apart ? half : 4);
   const bool live = 8 * sub < D;
+  const int turned = half - 4 * sub;  // how many of this lane's pairs turn: all from 4 on, none from 0 down
   pdl_trigger();
   pdl_wait();
   for (int i = threadIdx.x; i < 16 * G; i += kWarps * 32) {
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
               xs[q] = masked<T>(xs[q], i0 + q < count);
               F2 t[4];
               unpack<T, kPairs>(in[q], t);
-              turn(t, c, s, ns);
+              turn<kWhole>(t, c, s, ns, turned);
               unpack<T, kPairs>(xs[q], xv);
 #pragma unroll
               for (int i = 0; i < 4; ++i) t[i] = t[i] * scale[i];
@@ -318,9 +330,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
             if constexpr (!kBackward) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) f[i] = f[i] * rr * scale[i];
-              turn(f, c, s, ns);
+              turn<kWhole>(f, c, s, ns, turned);
             } else {
-              turn(f, c, s, ns);  // dz
+              turn<kWhole>(f, c, s, ns, turned);  // dz
               const float mean = dot[q] * r * a.inv_dim;  // mean(w dz xh)
               const F2 less = f2(-mean, -mean);
               F2 xv[4];
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(co
               }
             }
           } else {
-            turn(f, c, s, ns);
+            turn<kWhole>(f, c, s, ns, turned);
           }
           if (i0 + q < count) store8<T, kVec>(dst, gap, pack<T, kPairs>(f));
           dst += dst_step;
@@ -445,10 +457,14 @@ static int lanes_per_row(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : 32); }
 
 template <typename T, int G, bool kPairs, bool kVec>
 static int launch_t(const RopeArgs& a, bool backward, dim3 blocks, cudaStream_t st) {
+  auto go = [&](auto kern) { launch_overlapped(kern, blocks, rotary::kWarps * 32, st, a); };
+  // forms of their own where the whole row is turned: with one form that tests for it, the backward of 19982 tokens x 40
+  // heads x 64 took 94 us instead of 89, the forward 49.5 instead of 48.6
+  const bool whole = 2 * a.pairs == a.D;
   if (backward)
-    launch_overlapped(rotary::rope_kernel<T, G, kPairs, kVec, true>, blocks, rotary::kWarps * 32, st, a);
+    whole ? go(rotary::rope_kernel<T, G, kPairs, kVec, true, true>) : go(rotary::rope_kernel<T, G, kPairs, kVec, true, false>);
   else
-    launch_overlapped(rotary::rope_kernel<T, G, kPairs, kVec, false>, blocks, rotary::kWarps * 32, st, a);
+    whole ? go(rotary::rope_kernel<T, G, kPairs, kVec, false, true>) : go(rotary::rope_kernel<T, G, kPairs, kVec, false, false>);
   return check_launch("rope_kernel");
 }
 

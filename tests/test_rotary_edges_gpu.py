@@ -1,9 +1,11 @@
 """Edges of q/k normalisation with rotary positions (rotary.qk_norm_rope): eps = 0 with heads that leave lanes and steps
-without a row.
+without a row, and infinities and NaN among the elements that pass through.
 
 Tolerances, with u = 2^-24: a scale's gradient sums n products of a turned gradient (40 u of its pair's length) with a
 normalised value (20 u of itself), so it is off by at most (n + 64) u of their sizes; dx has 64 u of its terms' sizes;
-half a step of the output's type comes on top."""
+half a step of the output's type comes on top. Where a value has to be untouched by a neighbour, bits are compared."""
+import math
+
 import pytest
 import torch
 
@@ -59,3 +61,64 @@ def test_gradients_without_eps(cuda, B, H, KV, L, D, dtype):
         s = size * w64.abs()
         far = 64 * U * r * (s + xh.abs() * (s * xh.abs()).mean(-1, keepdim=True))
         _close(dx, want, far + HALF_STEP[dtype] * (want.abs() + far) + TINY[dtype])
+
+
+PARTLY = [(96, (32, 32), True), (96, (32, 32), False), (200, (30, 70), True), (16, (6,), True), (16, (8,), False),
+          (256, (2,), True), (72, (24, 24), False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,axes,interleaved", PARTLY, ids=str)
+def test_elements_that_pass_through_are_left_alone(cuda, D, axes, interleaved, dtype):
+    """Without a norm, an infinity or NaN past the rotated elements comes out as it went in and reaches no other
+    element, in either direction."""
+    B, H, L, r = 2, 5, 11, sum(axes)
+    g = torch.Generator().manual_seed(43)
+    x = torch.randn(B, H, L, D, generator=g).to(dtype).to(cuda)
+    dy = torch.randn(B, H, L, D, generator=g).to(dtype).to(cuda)
+    pos = torch.randint(1, 300, (L, len(axes)), generator=g).to(cuda)
+    mark = torch.zeros(B, H, L, D, dtype=torch.bool)
+    for i, v in enumerate((math.inf, -math.inf, math.nan)):
+        mark.view(-1, D)[i::3, r + i % (D - r)] = True
+        mark.view(-1, D)[i::7, D - 1] = True
+    mark = mark.to(cuda)
+    bad = torch.tensor([math.inf, -math.inf, math.nan]).to(dtype).to(cuda)[torch.arange(B * H * L, device=cuda) % 3]
+    bad = bad.view(B, H, L, 1).expand(B, H, L, D)
+
+    def both(x, dy):
+        x = x.detach().clone().requires_grad_(True)
+        y, _ = rotary.qk_norm_rope(x, None, pos, axes, interleaved=interleaved)
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    y0, d0 = both(x, dy)
+    y1, d1 = both(torch.where(mark, bad, x), torch.where(mark, bad, dy))
+    for base, got in ((y0, y1), (d0, d1)):
+        assert torch.equal(base[~mark], got[~mark])
+        assert torch.equal(got[mark].nan_to_num(7.0, 8.0, 9.0), bad[mark].nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("D,axes,interleaved", PARTLY, ids=str)
+def test_norm_with_an_infinite_element_that_passes_through(cuda, D, axes, interleaved):
+    """The norm takes such a row's finite elements to 0 (they are divided by an infinite root) and leaves inf / inf, a
+    NaN, in its own place alone. An infinite gradient of one such element makes that element's scale gradient
+    infinite and no other's."""
+    r = sum(axes)
+    g = torch.Generator().manual_seed(44)
+    x = torch.randn(1, 2, 3, D, generator=g).to(cuda)
+    x[0, 1, 1, r] = math.inf
+    pos = torch.randint(1, 300, (3, len(axes)), generator=g).to(cuda)
+    w = torch.ones(D, device=cuda)
+    y, _ = rotary.qk_norm_rope(x, None, pos, axes, q_scale=w, interleaved=interleaved)
+    row = y[0, 1, 1]
+    assert bool(torch.isnan(row[r])) and bool((row[torch.arange(D, device=cuda) != r] == 0).all())
+    assert bool(torch.isfinite(y[0, 0]).all())
+
+    x = torch.randn(1, 2, 3, D, generator=g).to(cuda)
+    w.requires_grad_(True)
+    y, _ = rotary.qk_norm_rope(x, None, pos, axes, q_scale=w, interleaved=interleaved)
+    dy = torch.randn(1, 2, 3, D, generator=g).to(cuda)
+    base = torch.autograd.grad(y, w, dy, retain_graph=True)[0]
+    dy[0, 1, 2, r] = math.inf
+    dw = torch.autograd.grad(y, w, dy)[0]
+    others = torch.arange(D, device=cuda) != r
+    assert torch.equal(dw[others], base[others]) and bool(torch.isinf(dw[r]))
