@@ -94,7 +94,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     bfloat16); grads: the same shapes, one dtype; exp_avgs, exp_avg_sqs:
     float32. ``step`` counts from 1. ``grad_scale`` (one float32 value on the
     device) multiplies every gradient, for clipping or unscaling without a
-    pass of its own."""
+    pass of its own. No tensor may overlap another. Captured in a CUDA graph,
+    the launch keeps the ``step`` and ``lr`` of the capture in every replay."""
     found = _lists(params, [("grads", grads, None, False), ("exp_avgs", exp_avgs, torch.float32, False),
                             ("exp_avg_sqs", exp_avg_sqs, torch.float32, False)])
     if found:
@@ -137,7 +138,9 @@ class AdamW(torch.optim.Optimizer):
     or 8 chooses how both moments are held. Each group's parameters move in as
     few launches as their number asks for (one per 56 tensors), separately for
     each pair of parameter and gradient dtype. ``step(grad_scale=...)`` as
-    ``adamw_step``'s."""
+    ``adamw_step``'s. ``step`` refuses to be captured in a CUDA graph: the
+    step's number and bias corrections are arguments of the launch, and every
+    replay would repeat the captured ones."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32):
@@ -175,6 +178,12 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for index in set().union(*(map(_DEVICES, group["params"]) for group in self.param_groups)):
+            if index >= 0:
+                with ops._on(torch.device("cuda", index)):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW.step cannot be captured in a CUDA graph: every replay would take the "
+                                           "captured step's number and learning rate")
         for group in self.param_groups:
             lists: dict = {}
             for p in group["params"]:
