@@ -186,23 +186,27 @@ class AdamW(torch.optim.Optimizer):
                                            "captured step's number and learning rate")
         for group in self.param_groups:
             lists: dict = {}
+            bits = group["state_bits"]
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                if p.grad.is_sparse:
+                if grad.is_sparse:
                     raise RuntimeError("AdamW takes dense gradients")
                 st = self.state[p]
                 if not st:
-                    st.update(self._fresh(p, group["state_bits"]))
-                st["step"] += 1
-                lists.setdefault((p.device, p.dtype, p.grad.dtype, st["step"]), []).append((p, p.grad.contiguous(), st))
+                    st.update(self._fresh(p, bits))
+                key = (p.device, p.dtype, grad.dtype, st["step"] + 1)
+                lists.setdefault(key, []).append((p, grad.contiguous(), st))
             for (*_, step), items in lists.items():
                 ps, gs, sts = zip(*items)
                 more = dict(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                             weight_decay=group["weight_decay"], grad_scale=grad_scale)
-                if group["state_bits"] == 32:
+                if bits == 32:
                     adamw_step(ps, gs, [s["exp_avg"] for s in sts], [s["exp_avg_sq"] for s in sts], **more)
                 else:
                     adamw_step_8bit(ps, gs, *([s[k] for s in sts]
                                               for k in ("m_codes", "m_scales", "v_codes", "v_scales")), **more)
+                for st in sts:  # a call that was refused is not a step
+                    st["step"] = step
         return loss

@@ -1,4 +1,4 @@
-"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture."""
+"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture, refused steps."""
 import pytest
 import torch
 
@@ -34,3 +34,29 @@ def test_step_refuses_a_graph_capture(cuda, bits):
     assert torch.equal(p.detach(), before) and opt.state[p]["step"] == 1 and bool((other == 1).all())
     opt.step()
     assert opt.state[p]["step"] == 2 and not torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_refused_step_is_not_counted(cuda, bits):
+    """A call that is refused moves no step counter: the next one is the first step, bit for bit."""
+    a, b = _param(cuda, 37, 5), _param(cuda, 37, 5)
+    mine, fresh = (optim.AdamW([p], lr=1e-2, state_bits=bits) for p in (a, b))
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="grad_scale"):
+            mine.step(grad_scale=torch.ones(2, device=cuda))
+    mine.step()
+    fresh.step()
+    assert torch.equal(a, b) and mine.state[a]["step"] == fresh.state[b]["step"] == 1
+
+
+def test_only_what_moved_is_counted(cuda):
+    """Two launches of one step, the second one refused: the first one's parameters moved and are counted."""
+    good, bad = _param(cuda, 50), _param(cuda, 6, 8, dtype=torch.bfloat16)
+    bad.data = bad.data.t()
+    bad.grad = torch.ones(8, 6, device=cuda, dtype=torch.bfloat16)
+    before = good.detach().clone()
+    opt = optim.AdamW([good, bad], lr=1e-2)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        opt.step()
+    assert opt.state[good]["step"] == 1 and not torch.equal(good.detach(), before)
+    assert opt.state[bad]["step"] == 0
