@@ -32,12 +32,13 @@ def moment_scales(numel: int) -> int:
 
 
 # Whole lists at a time, without a loop of Python's own: a step over many small tensors is bound by this side.
-_DTYPES, _DEVICES = operator.attrgetter("dtype"), torch.Tensor.get_device
+_DTYPES, _SHAPES, _DEVICES = operator.attrgetter("dtype"), operator.attrgetter("shape"), torch.Tensor.get_device
 _NUMELS, _CONTIGUOUS, _ADDRESSES = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 
 def _lists(params, others):
-    """Checks the lists of one step: others is [(name, tensors, dtype or None for the first one's, scales)]; returns
+    """Checks the lists of one step: others is [(name, tensors, dtype or None for the first one's, scales)], the
+    gradients first, which have the parameters' shapes, where the rest have their numbers of elements; returns
     (device, elements of each parameter), or None where there is nothing to do."""
     n = len(params)
     for name, tensors, _, _ in others:
@@ -48,17 +49,19 @@ def _lists(params, others):
     ops._require_cuda(params[0], "params[0]")
     dev, index, numel = params[0].device, params[0].get_device(), list(map(_NUMELS, params))
     ops._dtype_code(params[0].dtype)
-    here, yes = [index] * n, [True] * n
+    here, yes, shapes = [index] * n, [True] * n, list(map(_SHAPES, params))
     for name, tensors, dtype, scales in (("params", params, None, False), *others):
         dtype = dtype or tensors[0].dtype
-        want = list(map(moment_scales, numel)) if scales else numel
+        size, want = (_SHAPES, shapes) if name in ("params", "grads") else (
+            _NUMELS, list(map(moment_scales, numel)) if scales else numel)
         if (list(map(_DTYPES, tensors)) != [dtype] * n or list(map(_DEVICES, tensors)) != here
-                or list(map(_NUMELS, tensors)) != want or list(map(_CONTIGUOUS, tensors)) != yes):
+                or (tensors is not params and list(map(size, tensors)) != want)
+                or list(map(_CONTIGUOUS, tensors)) != yes):
             i = next(i for i, t in enumerate(tensors) if t.dtype != dtype or t.get_device() != index
-                     or t.numel() != want[i] or not t.is_contiguous())
-            t = tensors[i]
-            raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {want[i]} elements; got {t.dtype} "
-                               f"on {t.device}, {tuple(t.shape)}, strides {t.stride()}")
+                     or size(t) != want[i] or not t.is_contiguous())
+            t, asked = tensors[i], f"shape {tuple(want[i])}" if want is shapes else f"{want[i]} elements"
+            raise RuntimeError(f"{name}[{i}] must be contiguous, {dtype} on {dev} with {asked}; got {t.dtype} on "
+                               f"{t.device}, {tuple(t.shape)}, strides {t.stride()}")
     return dev, numel
 
 

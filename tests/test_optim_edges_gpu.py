@@ -1,4 +1,4 @@
-"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture, refused steps."""
+"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture, refused steps, gradients of another shape."""
 import pytest
 import torch
 
@@ -60,3 +60,19 @@ def test_only_what_moved_is_counted(cuda):
         opt.step()
     assert opt.state[good]["step"] == 1 and not torch.equal(good.detach(), before)
     assert opt.state[bad]["step"] == 0
+
+
+def test_gradient_of_another_shape_is_refused(cuda):
+    """As many elements in another order are another tensor's gradient."""
+    p, g = torch.ones(3, 2, device=cuda), torch.ones(2, 3, device=cuda)
+    m, v = torch.zeros(3, 2, device=cuda), torch.zeros(3, 2, device=cuda)
+    with pytest.raises(RuntimeError, match=r"grads\[0\].*\(3, 2\).*\(2, 3\)"):
+        optim.adamw_step([p], [g], [m], [v], step=1, lr=1e-2)
+    with pytest.raises(RuntimeError, match=r"grads\[1\]"):
+        optim.adamw_step([p, p.clone()], [g.t().contiguous(), g.view(6)], [m, m.clone()], [v, v.clone()], step=1,
+                         lr=1e-2)
+    assert bool((p == 1).all()) and bool((m == 0).all())
+    z = lambda dt: torch.zeros(6, dtype=dt, device=cuda)  # noqa: E731
+    with pytest.raises(RuntimeError, match=r"grads\[0\]"):
+        optim.adamw_step_8bit([p], [g], [z(torch.int8)], [z(torch.float32)[:1]], [z(torch.uint8)],
+                              [z(torch.float32)[:1]], step=1, lr=1e-2)
