@@ -147,12 +147,18 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32):
-        if state_bits not in (32, 8):
-            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"expected lr, eps, weight_decay >= 0 and betas in [0, 1); got lr={lr} eps={eps} "
-                             f"weight_decay={weight_decay} betas={betas}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group):
+        """torch's, with the settings checked: the constructor's and the group's own."""
+        own = {**self.defaults, **param_group}
+        if own["state_bits"] not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {own['state_bits']}")
+        if not (own["lr"] >= 0 and own["eps"] >= 0 and own["weight_decay"] >= 0
+                and all(0 <= b < 1 for b in own["betas"])):
+            raise ValueError(f"expected lr, eps, weight_decay >= 0 and betas in [0, 1); got lr={own['lr']} "
+                             f"eps={own['eps']} weight_decay={own['weight_decay']} betas={own['betas']}")
+        super().add_param_group(param_group)
 
     def _fresh(self, p: torch.Tensor, bits: int) -> dict:
         if bits == 32:

@@ -1,4 +1,5 @@
-"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture, refused steps, gradients of another shape."""
+"""Edges of the AdamW operators (optim): a step inside a CUDA graph capture, refused steps, gradients of another shape,
+groups with their own settings."""
 import pytest
 import torch
 
@@ -76,3 +77,19 @@ def test_gradient_of_another_shape_is_refused(cuda):
     with pytest.raises(RuntimeError, match=r"grads\[0\]"):
         optim.adamw_step_8bit([p], [g], [z(torch.int8)], [z(torch.float32)[:1]], [z(torch.uint8)],
                               [z(torch.float32)[:1]], step=1, lr=1e-2)
+
+
+def test_group_settings_are_checked(cuda):
+    """A group's own settings meet the checks of the constructor's."""
+    for more in (dict(state_bits=16), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0)),
+                 dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            optim.AdamW([{"params": [_param(cuda, 4)], **more}])
+        opt = optim.AdamW([_param(cuda, 4)])
+        with pytest.raises(ValueError):
+            opt.add_param_group({"params": [_param(cuda, 4)], **more})
+        assert len(opt.param_groups) == 1
+    a, b = _param(cuda, 300, seed=1), _param(cuda, 300, seed=1)
+    opt = optim.AdamW([{"params": [a], "state_bits": 8}, {"params": [b]}], lr=1e-2)
+    opt.step()
+    assert "m_codes" in opt.state[a] and "exp_avg" in opt.state[b]
