@@ -84,7 +84,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     of a fused [2F, K] weight are read in place). activation: "silu", "gelu"
     or "gelu_tanh". Products accumulate in float32 and the result is rounded
     once. Differentiable in every tensor; a call that needs a gradient keeps
-    both projections in float32 (8 bytes for each element of the result)."""
+    both projections in float32 (8 bytes for each element of the result).
+    Forward-mode derivatives are refused."""
     ops._require_cuda(x, "x")
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"x must be float16 or bfloat16, got {x.dtype}")
@@ -111,7 +112,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
         raise RuntimeError(f"at most 2^30 tokens, got {x2.shape[0]}")
     args = (_rows(x2), _rows(w_gate), _rows(w_up), b_gate.contiguous() if b_gate is not None else None,
             b_up.contiguous() if b_up is not None else None)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
+    if (torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args])) or ops._has_tangent(*args):
         h = _GatedLinear.apply(*args, ACTIVATIONS[activation])
     else:
         h = _forward(*args, ACTIVATIONS[activation], False)[0]

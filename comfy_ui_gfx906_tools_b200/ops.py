@@ -28,6 +28,7 @@ import contextlib
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -61,6 +62,13 @@ def _on(device: torch.device):
     """The context of a call on `device`: nothing to do where it is current, which entering torch.cuda.device would
     find out in some microseconds."""
     return _HERE if device.index == _CURRENT_DEVICE() else torch.cuda.device(device)
+
+
+def _has_tangent(*tensors) -> bool:
+    """Whether a forward-mode derivative is under way in any of the tensors (or None). An operator without one has to
+    go through its autograd function then, which refuses; called past it, it would lose the tangent in silence."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
 
 
 def _require_cuda(t: torch.Tensor, name: str):

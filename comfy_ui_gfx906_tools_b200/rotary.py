@@ -129,7 +129,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     pair (``flux_dit.apply_rope``'s layout), else element i and
     i + sum(axes_dims) / 2. Pair j of an axis of d elements turns by
     position * theta^(-2j/d). q_scale / k_scale [D]: the norm's scale (None:
-    that tensor is not normalised). Differentiable in q, k and the scales."""
+    that tensor is not normalised). Differentiable in q, k and the scales
+    (backward only; forward-mode derivatives are refused)."""
     index, dt, shape = q.get_device(), q.dtype, q.shape
     if index < 0:
         ops._require_cuda(q, "q")
@@ -172,7 +173,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         q_scale, k_scale = (s.contiguous() if s is not None else None for s in (q_scale, k_scale))
     q, k = _rows(q), _rows(k) if k is not None else None
     call = (code, scale_code, pos_code, kv, (axes, n, float(theta), int(interleaved), float(eps)))
-    if torch.is_grad_enabled() and (q.requires_grad or any([t is not None and t.requires_grad
-                                                            for t in (k, q_scale, k_scale)])):
+    if ((torch.is_grad_enabled() and (q.requires_grad or any([t is not None and t.requires_grad
+                                                             for t in (k, q_scale, k_scale)])))
+            or ops._has_tangent(q, k, positions, q_scale, k_scale)):
         return _QkNormRope.apply(q, k, positions, q_scale, k_scale, ps, call)
     return _forward(q, k, positions, ps, q_scale, k_scale, call)

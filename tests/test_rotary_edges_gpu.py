@@ -122,3 +122,16 @@ def test_norm_with_an_infinite_element_that_passes_through(cuda, D, axes, interl
     dw = torch.autograd.grad(y, w, dy)[0]
     others = torch.arange(D, device=cuda) != r
     assert torch.equal(dw[others], base[others]) and bool(torch.isinf(dw[r]))
+
+
+def test_forward_mode_is_refused(cuda):
+    """No tangent is lost in silence: there is no forward-mode derivative, and a call with one says so."""
+    x, pos = torch.randn(1, 2, 3, 64, device=cuda), torch.zeros(3, 1, device=cuda)
+    w = torch.ones(64, device=cuda)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward"):
+            rotary.qk_norm_rope(dual, None, pos, (64,))
+        with pytest.raises(RuntimeError, match="forward"):
+            rotary.qk_norm_rope(x, None, pos, (64,), q_scale=torch.autograd.forward_ad.make_dual(w, w))
+        rotary.qk_norm_rope(x, None, pos, (64,))  # a call without a tangent goes through
