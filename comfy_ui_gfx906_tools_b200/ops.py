@@ -82,26 +82,38 @@ def _require_cuda(t: torch.Tensor, name: str):
 # ---------------------------------------------------------------------------
 _ws_lock = threading.Lock()
 _workspaces: dict = {}
+_retired: list = []  # (device index, workspace): outgrown ones, which a CUDA graph captured earlier may still name
 
 
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor | None:
-    if nbytes == 0:
-        return None
+def _cached(cache: dict, device: torch.device, stream: int, nbytes: int, make) -> torch.Tensor:
+    """The workspace of (device, stream), at least nbytes long. One that is outgrown stays allocated: a replayed graph
+    writes where it was captured. The next one is twice as long or longer, so all of them together take less than twice
+    the last one's memory. A workspace that has to be made inside a capture belongs to that graph alone: its memory is
+    the graph's, and it is filled by a replay, not before one."""
     key = (device.index, stream)
     with _ws_lock:
-        ws = _workspaces.get(key)
+        ws = cache.get(key)
         if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                return make(nbytes, dtype=torch.uint8, device=device)
+            size = max(nbytes, 1 << 20)
+            if ws is not None:
+                _retired.append((device.index, ws))
+                size = max(size, 2 * ws.numel())
+            ws = cache[key] = make(size, dtype=torch.uint8, device=device)
         return ws
 
 
+def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor | None:
+    return _cached(_workspaces, device, stream, nbytes, torch.zeros) if nbytes else None
+
+
 def _rearm_workspaces(device: torch.device):
-    """Zero every cached split-K workspace of `device`: after a kernel gave up
-    in a bounded wait, its row blocks' arrival counters may be left non-zero,
-    and a later call sharing the workspace would sum the wrong segments."""
+    """Zero every split-K workspace of `device`: after a kernel gave up in a
+    bounded wait, its row blocks' arrival counters may be left non-zero, and a
+    later call sharing the workspace would sum the wrong segments."""
     with _ws_lock:
-        for (idx, _), ws in _workspaces.items():
+        for idx, ws in [(key[0], ws) for key, ws in _workspaces.items()] + _retired:
             if idx == device.index:
                 ws.zero_()
 
@@ -551,20 +563,13 @@ def int4_linear(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, 
     return out.reshape(*shape[:-1], w_packed.shape[0])
 
 
-_exact_ws_lock = threading.Lock()
 _exact_workspaces: dict = {}
 
 
 def _exact_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of the integer-exact GEMM per (device, stream): the e5m2 copy of
     A and its transposed scales, rewritten by every call (no state kept)."""
-    key = (device.index, stream)
-    with _exact_ws_lock:
-        ws = _exact_workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _exact_workspaces[key] = ws
-        return ws
+    return _cached(_exact_workspaces, device, stream, nbytes, torch.empty)
 
 
 def gemm_int4(A_packed: torch.Tensor, A_scale: torch.Tensor, B_packed: torch.Tensor, B_scale: torch.Tensor,

@@ -1,8 +1,11 @@
-"""Edges of the gated feed-forward product (gated.gated_linear): forward-mode derivatives."""
+"""Edges of the gated feed-forward product (gated.gated_linear): forward-mode derivatives, a workspace
+that grows after a CUDA graph was captured, and one that is made inside a capture."""
+import math
+
 import pytest
 import torch
 
-from comfy_ui_gfx906_tools_b200 import gated
+from comfy_ui_gfx906_tools_b200 import gated, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +20,64 @@ def test_forward_mode_is_refused(cuda):
         with pytest.raises(RuntimeError, match="forward"):
             gated.gated_linear(x, w, torch.autograd.forward_ad.make_dual(w, w))
         gated.gated_linear(x, w, w)  # a call without a tangent goes through
+
+
+def _cut(cuda, M, K, F, seed):
+    """Operands of a product whose few tiles are cut along K, which takes a workspace."""
+    from comfy_ui_gfx906_tools_b200 import _lib
+    assert _lib.load().gated_linear_workspace_bytes(M, K, F) > 1 << 18
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g).bfloat16().to(cuda)
+    return x, *((torch.randn(F, K, generator=g) / math.sqrt(K)).bfloat16().to(cuda) for _ in range(2))
+
+
+def _captured(stream, args):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        h = gated.gated_linear(*args)
+    return graph, h
+
+
+def test_a_graph_outlives_a_grown_workspace(cuda):
+    """A larger call on the stream of a capture replaces the workspace; the graph still joins its tiles in its own, and
+    writes into nobody else's memory."""
+    small, large = _cut(cuda, 200, 2048, 136, 61), _cut(cuda, 700, 6400, 72, 62)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    ops._workspaces.pop((0, side.cuda_stream), None)
+    with torch.cuda.stream(side):
+        want = gated.gated_linear(*small)
+        held = ops._workspaces[(0, side.cuda_stream)].data_ptr()
+    side.synchronize()
+    graph, h = _captured(side, small)
+    with torch.cuda.stream(side):
+        gated.gated_linear(*large)
+        assert ops._workspaces[(0, side.cuda_stream)].data_ptr() != held
+        # whatever is allocated from now on is not the graph's
+        mine = [torch.full((1 << 20,), 0x5A, dtype=torch.uint8, device=cuda) for _ in range(64)]
+    side.synchronize()
+    for _ in range(3):
+        h.zero_()
+        graph.replay()
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(h, want)
+    assert all(bool((t == 0x5A).all()) for t in mine)
+
+
+def test_a_workspace_made_in_a_capture_is_the_graphs_own(cuda):
+    """No call before the capture: eager calls on the same stream, before any replay, have a zeroed workspace too."""
+    args = _cut(cuda, 200, 2048, 136, 63)
+    want = gated.gated_linear(*args)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    ops._workspaces.pop((0, side.cuda_stream), None)
+    graph, h = _captured(side, args)
+    with torch.cuda.stream(side):
+        eager = gated.gated_linear(*args)
+    side.synchronize()
+    assert torch.equal(eager, want)
+    for _ in range(2):
+        h.zero_()
+        graph.replay()
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(h, want)
