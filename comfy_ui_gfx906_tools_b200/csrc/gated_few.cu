@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
     }
     __syncwarp();
   } else if (warp == 5) {
+    pdl_wait();  // its waits are limited, and the stream's previous kernel is not
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t id = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(a.columns >> 3) << 17) |
                         ((uint32_t)(kFewTile >> 4) << 24);

@@ -95,6 +95,8 @@ struct TcArgs {
   const void* bias1;
   float* save;          // forward: g, u
   int wide;             // rows of every output are 32-byte aligned
+  int overlap;          // the stream's next kernel may start while this one ends
+  unsigned long long wait_ns;  // limit of the waits for a whole contraction, and for the kernel's last MMA
   int* status_host;
 };
 
@@ -239,7 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
   cluster_sync_all();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_base;
-  pdl_trigger();
+  if (a.overlap) pdl_trigger();
 
   bool ok = true;
   if (warp == kLoadWarp) {
@@ -295,6 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
+    pdl_wait();  // its waits are limited, and the stream's previous kernel is not
     if (cr == 0) {
       constexpr uint32_t kId = instruction_desc<T, kRole>();
       constexpr uint64_t kStepA = kRole == kWeightGrad ? 128 : 2, kStepB = kRole == kForward ? 2 : 128;  // 16 of K
@@ -374,7 +377,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
       if (lane == 0) commit(drain);
       __syncwarp();
     }
-    if (!mbar_wait(drain, 0, kDevErrMmaBarrierTimeout)) ok = false;
+    // CTA 1's warp comes here at once and waits as long as the kernel runs
+    if (!mbar_wait_for(drain, 0, kDevErrMmaBarrierTimeout, a.wait_ns)) ok = false;
   } else {
     const int quadrant = warp & 3, side = warp >> 2;  // 32 TMEM lanes; which half of the columns
     pdl_wait();
@@ -389,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
       for (int b = 0; b < kBlocks; ++b) {
         const int acc = kBlocks == 2 ? b : n & 1;
         const int row = row0 + b * kBlockRows;
-        if (!mbar_wait(&acc_full[acc], (kBlocks == 2 ? n : n >> 1) & 1, kDevErrEpilogueBarrierTimeout)) {
+        if (!mbar_wait_for(&acc_full[acc], (kBlocks == 2 ? n : n >> 1) & 1, kDevErrEpilogueBarrierTimeout, a.wait_ns)) {
           ok = false;
           break;
         }
@@ -429,7 +433,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
           // The parts come through this warp's 16 KB of the stages' memory, which is free: a pair's cut tile is the
           // last thing it does, and its loads and MMAs (the second block's too) are done. Two parts: the other one is
           // added to the registers (a sum of two has no order). More: all of them, from the first on.
-          if (kBlocks == 2 && b == 0 && !mbar_wait(&acc_full[1], n & 1, kDevErrEpilogueBarrierTimeout)) {
+          if (kBlocks == 2 && b == 0 &&
+              !mbar_wait_for(&acc_full[1], n & 1, kDevErrEpilogueBarrierTimeout, a.wait_ns)) {
             ok = false;
             break;
           }
@@ -499,6 +504,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ke
   if (warp == kMmaWarp) tc::tmem_dealloc<2>(tmem, 512);
 }
 
+// Limits of a launch whose pairs take `units` tiles each of `stages` along the contraction. A wait for one stage has the
+// usual limit. A wait for a whole contraction, or for the kernel's last MMA, may rightly take longer: it has 4 us a stage
+// (one takes 0.4 to 1 us) and 0.1 ms a tile besides. A pipeline that is stuck ends earlier all the same, by the stage's
+// limit: every wait ends once one of them has given up. A launch of more than some 25 ms does not let the stream's next
+// kernel in early, whose own waits would count the rest of this one.
+static void set_limits(TcArgs& a, long long units, long long stages) {
+  const unsigned long long longest = (unsigned long long)units * (4000ull * (unsigned long long)stages + 100000ull);
+  a.wait_ns = kWaitTimeoutNs + longest;
+  a.overlap = longest < 100000000ull;
+}
+
 template <typename T, int kRole, int kAct, int kBlocks>
 static int launch_pair_blocks(TcArgs& a, cudaStream_t st, int sms) {
   constexpr int kSmemBytes = Ring<kBlocks>::kSmemBytes;
@@ -531,7 +547,10 @@ static int launch_pair_blocks(TcArgs& a, cudaStream_t st, int sms) {
   // a pair takes at most one part of a cut tile (it uses the stages' memory to join them)
   if (a.cut * a.parts > pairs_at_once[dev]) a.parts = 1;
   const int units = a.whole + a.cut * a.parts;
-  cfg.gridDim = dim3(2 * (units < pairs_at_once[dev] ? units : pairs_at_once[dev]));
+  const int pairs = units < pairs_at_once[dev] ? units : pairs_at_once[dev];
+  const long long steps = (a.depth + kStageK - 1) / kStageK;
+  set_limits(a, (units + pairs - 1) / pairs, kRole == kInputGrad ? 2 * steps : steps);
+  cfg.gridDim = dim3(2 * pairs);
   a.status_host = host_status_word(dev);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(GFX_ERR_CUDA, "gated pair_kernel launch: %s", cudaGetErrorString(e));

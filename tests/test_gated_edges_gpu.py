@@ -1,5 +1,5 @@
 """Edges of the gated feed-forward product (gated.gated_linear): forward-mode derivatives, a workspace
-that grows after a CUDA graph was captured, and one that is made inside a capture."""
+that grows after a CUDA graph was captured, one that is made inside a capture, and one launch of several seconds."""
 import math
 
 import pytest
@@ -81,3 +81,28 @@ def test_a_workspace_made_in_a_capture_is_the_graphs_own(cuda):
         graph.replay()
         torch.cuda.synchronize(cuda)
         assert torch.equal(h, want)
+
+
+def test_a_launch_of_several_seconds(cuda):
+    """5.6e15 operations in one launch, longer than the limit of a wait for one stage, with a call right behind it: both
+    are right and no wait gave up. Operands are +-1 and +-2^-9, whose sums are exact in float32, so a sampled result is
+    off by its activation (1e-5 of it) and its own rounding alone."""
+    M, K, F = 65536, 163840, 131072
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(cuda)[0] < 100 * 2 ** 30:
+        pytest.skip("needs 100 GB of free memory")
+    g = torch.Generator(device=cuda).manual_seed(71)
+    x = torch.empty(M, K, device=cuda, dtype=torch.bfloat16).bernoulli_(0.5, generator=g).mul_(2).sub_(1)
+    w = torch.empty(F, K, device=cuda, dtype=torch.bfloat16).bernoulli_(0.5, generator=g).sub_(0.5).mul_(2.0 ** -8)
+    with torch.no_grad():
+        h = gated.gated_linear(x, w, w)
+        few = gated.gated_linear(x[:40], w[:520], w[:520])
+    rows, cols = (torch.randperm(n, generator=g, device=cuda)[:128] for n in (M, F))
+    gate = x[rows].double() @ w[cols].double().T
+    want = gate * torch.sigmoid(gate) * gate
+    got = h[rows][:, cols].double()
+    assert bool(((got - want).abs() <= (2.0 ** -8 + 1e-5) * want.abs()).all())
+    assert torch.equal(few, h[:40, :520])
+    assert ops.device_status(cuda) == 0
+    del x, w, h
+    torch.cuda.empty_cache()
