@@ -1,5 +1,6 @@
-"""Edges of the gated feed-forward product (gated.gated_linear): forward-mode derivatives, a workspace
-that grows after a CUDA graph was captured, one that is made inside a capture, and one launch of several seconds."""
+"""Edges of the gated feed-forward product (gated.gated_linear): far negative gates against their own size,
+forward-mode derivatives, a workspace that grows after a CUDA graph was captured, one that is made inside a capture, and
+one launch of several seconds."""
 import math
 
 import pytest
@@ -8,6 +9,75 @@ import torch
 from comfy_ui_gfx906_tools_b200 import gated, ops
 
 pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}  # half the smallest step
+ACTS = list(gated.ACTIVATIONS)
+K2 = 2 * math.sqrt(2 / math.pi)
+
+
+def _act(g, name):
+    """a, a' as its two terms, and the size of the exponential's argument, in 64 bits without cancellation."""
+    if name == "silu":
+        s, t, e = torch.sigmoid(g), torch.sigmoid(-g), g.abs()
+        return g * s, (s, g * s * t), e
+    if name == "gelu":
+        c, e = 0.5 * torch.erfc(-g / math.sqrt(2)), g * g / 2
+        return g * c, (c, g * torch.exp(-e) / math.sqrt(2 * math.pi)), e
+    y = K2 * (g + 0.044715 * g ** 3)
+    s, t = torch.sigmoid(y), torch.sigmoid(-y)
+    return g * s, (s, g * s * t * K2 * (1 + 3 * 0.044715 * g * g)), y.abs()
+
+
+def _relative(e):
+    """How far an activation may be off, of its value, where its exponential's argument has the size e.
+
+    CUDA's fast exponential is documented to 2 + 1.173 e steps (2 u each), its fast division to 2; the argument has up
+    to four roundings (u of e each, which the exponential turns into a relative error), the rest some ten (u each).
+    Phi's polynomial is within 2e-6."""
+    return (2 * (2 + 1.173 * e) + 4 + 4 * e + 10) * U + 2e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [1, 40, 160])
+def test_far_gates_keep_their_precision(cuda, act, M, dtype):
+    """Every gate is one exact product and every up projection is 2 or 1, so a result is off by its activation and its
+    own rounding alone, of its own size, however small that is; the same for dg and du, which one token's weight
+    gradients show as they are (a sum of one product with 1). a' is a sum of two terms: the error is of their sizes."""
+    K, F = 72, 8192
+    gates = torch.cat([-torch.linspace(0, 6, F // 2), -torch.linspace(6, 100, F // 2)]).to(dtype)
+    x, wg, wu = torch.zeros(M, K, dtype=dtype), torch.zeros(F, K, dtype=dtype), torch.zeros(F, K, dtype=dtype)
+    x[:, 0] = 1 - 0.25 * (torch.arange(M) % 2)
+    x[:, 1] = 1
+    wg[:, 0] = gates
+    wu[:, 1] = 1 + torch.arange(F) % 2
+    x, wg, wu = (t.to(cuda) for t in (x, wg, wu))
+    g = x[:, :1].double() * wg[:, 0].double()
+    u = wu[:, 1].double().expand(M, F)
+    a, terms, e = _act(g, act)
+    off = _relative(e)
+    e16, tiny = HALF_STEP[dtype], TINY[dtype]
+
+    def close(got, want, size):
+        far = off[:got.shape[0]] * size
+        far = far + e16 * (want.abs() + far) + tiny
+        d = (got.double() - want).abs()
+        i = int((d / far).argmax())
+        assert bool((d <= far).all()), (f"{float((d / far).max()):.3g} of what is allowed at gate "
+                                        f"{float(g.expand_as(d).reshape(-1)[i]):.6g}: {float(got.reshape(-1)[i]):.6g}, "
+                                        f"want {float(want.reshape(-1)[i]):.6g}")
+
+    with torch.no_grad():
+        close(gated.gated_linear(x, wg, wu, activation=act), a * u, (a * u).abs())
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
+    h = gated.gated_linear(*leaves, activation=act)
+    close(h.detach(), a * u, (a * u).abs())
+    if M == 1:
+        dwg, dwu = torch.autograd.grad(h, leaves[1:], torch.ones_like(h))
+        close(dwg[:, 0][None], u * sum(terms), u * sum(t.abs() for t in terms))
+        close(dwu[:, 1][None], a, a.abs())
 
 
 def test_forward_mode_is_refused(cuda):
