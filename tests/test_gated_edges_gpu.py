@@ -1,6 +1,6 @@
 """Edges of the gated feed-forward product (gated.gated_linear): far negative gates against their own size,
-forward-mode derivatives, a workspace that grows after a CUDA graph was captured, one that is made inside a capture, and
-one launch of several seconds."""
+joins of a cut contraction with many tokens, forward-mode derivatives, a workspace that grows after a CUDA graph was
+captured, one that is made inside a capture, and one launch of several seconds."""
 import math
 
 import pytest
@@ -78,6 +78,35 @@ def test_far_gates_keep_their_precision(cuda, act, M, dtype):
         dwg, dwu = torch.autograd.grad(h, leaves[1:], torch.ones_like(h))
         close(dwg[:, 0][None], u * sum(terms), u * sum(t.abs() for t in terms))
         close(dwu[:, 1][None], a, a.abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,F", [(65, 1032, 264), (100, 2056, 520), (128, 4104, 136), (128, 1544, 1000), (77, 776, 72)])
+def test_few_tokens_with_a_cut_contraction(cuda, M, K, F, dtype):
+    """65 to 128 tokens and a contraction that is cut among the CTAs of a cluster. A projection of K + 1 terms is off by
+    at most 2 u each of the terms' sizes; the activation (slope 1.2 at most) and the product carry that on, and the
+    result has half a step of its own."""
+    g = torch.Generator().manual_seed(51)
+    x = torch.randn(M, K, generator=g).to(dtype).to(cuda)
+    wg, wu = ((torch.randn(F, K, generator=g) / math.sqrt(K)).to(dtype).to(cuda) for _ in range(2))
+    bg, bu = ((torch.randn(F, generator=g) * 0.3).to(dtype).to(cuda) for _ in range(2))
+    X, G, W, cg, cu = (t.double() for t in (x, wg, wu, bg, bu))
+    gate, up = X @ G.T + cg, X @ W.T + cu
+    n = 2 * U * (K + 2)
+    far_g, far_u = n * (X.abs() @ G.abs().T + cg.abs()), n * (X.abs() @ W.abs().T + cu.abs())
+    for act in ACTS:
+        a, _, e = _act(gate, act)
+        far_a = 1.2 * far_g + _relative(e) * a.abs()
+        far = far_a * (up.abs() + far_u) + a.abs() * far_u
+        far = far + HALF_STEP[dtype] * ((a * up).abs() + far) + TINY[dtype]
+        with torch.no_grad():
+            h = gated.gated_linear(x, wg, wu, bg, bu, activation=act)
+            assert torch.equal(h, gated.gated_linear(x, wg, wu, bg, bu, activation=act))
+        d = (h.double() - a * up).abs()
+        assert bool((d <= far).all()), f"{act}: off by up to {float((d / far).max()):.3g} of what is allowed"
+    # the same sums are kept for a backward
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+    assert torch.equal(gated.gated_linear(*leaves, activation=ACTS[-1]), h)
 
 
 def test_forward_mode_is_refused(cuda):
