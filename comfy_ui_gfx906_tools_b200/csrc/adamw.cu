@@ -28,7 +28,10 @@
 // approximate roots, off by 2^-23, and decides a code by them unless the root
 // lies so near the middle between two codes that this error could matter; a
 // lane that sees such an element (one in five thousand), or a vanishing root,
-// does its eight elements again exactly. Codes are turned into floats and back
+// does its eight elements again exactly. The parameters' move, which no code
+// depends on, takes them too: it is off by some 2^-22 of itself there, and exact
+// to the division's rounding in a tensor's ragged end and in the 32-bit form, so
+// a parameter's last bit may depend on its place in the tensor. Codes are turned into floats and back
 // by adding 2^23 and 1.5 * 2^23, not by the quarter-rate conversions. Packed
 // pairs of floats are not used here: the compiler fuses a packed product and
 // sum, and the moments' definition rounds both.

@@ -119,7 +119,9 @@ int launch_moment_values(const void* codes, const float* scale, float* out, long
 // q/k normalisation with rotary positions -- rotary.cu
 constexpr int kRopeMaxDim = 256;
 constexpr int kRopeMaxAxes = 8;
-constexpr int kRopeMaxBlocks = 148 * 8;  // blocks of one launch; the backward's partial sums have this many rows
+// Most blocks of a backward that sums scale gradients, and the rows of its partial sums: 8 an SM of a B200. A constant,
+// because the workspace's size is asked for without a device.
+constexpr int kRopeMaxBlocks = 148 * 8;
 enum : int { kPositionF32 = 0, kPositionI32 = 1, kPositionI64 = 2 };
 struct RopeTensor {
   const void* in;   // forward: x; backward: dy          strides: batch, head, token (elements)

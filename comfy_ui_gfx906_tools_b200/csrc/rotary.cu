@@ -27,8 +27,10 @@
 // Arithmetic is on pairs of floats, one instruction for two. Measured on B200:
 // forward of 4608 tokens x 48 heads x 128 in bfloat16 (113 MB) 21 us, 5.4 TB/s;
 // 19982 tokens x 40 heads x 64, forward 48 us (205 MB), backward 89 us (307 MB).
-// What bounds it is the issue of the 16-bit conversions and the reductions
-// against the latency of the loads, at 32 warps an SM (16 in the backward).
+// The forward runs at 32 warps an SM and issues 64% of the cycles, in 16-bit
+// conversions and reductions between the loads. The backward waits on loads: its
+// registers (109 to 123) leave 16 warps an SM, 47% of the cycles issue, and
+// nothing is in flight while a warp works on the rows that it has.
 #include <math.h>
 #include <string.h>
 
@@ -191,6 +193,7 @@ __device__ __forceinline__ void turn(F2 (&f)[4], const F2 (&c)[2], const F2 (&s)
 // scale), out is dx, and each block leaves its sums of dz xh in partial
 // [block][2][D] (q, then k).
 // kVec: every row starts at a multiple of 16 bytes. kWhole: no pair passes through.
+// Eight blocks an SM hold the forward to 64 registers: 16-bit rows fit, float32 ones spill 4 to 36 bytes a thread.
 template <typename T, int G, bool kPairs, bool kVec, bool kBackward, bool kWhole>
 __global__ void __launch_bounds__(kWarps * 32, kBackward ? 4 : 8) rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kRows = 32 / G, kLanePairs = 4 * G;
