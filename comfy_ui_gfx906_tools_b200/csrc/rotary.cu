@@ -438,9 +438,12 @@ void rope_frequencies(RopeArgs* a, const int* axes_dims, int n_axes, double thet
   a->axes = n_axes;
 }
 
-// A block's four warps hold 4 tokens, or fewer with several warps a token where that leaves less than six blocks an SM
-// (at twelve, 4608 tokens of 48 heads took 23 us instead of 21); a lone token's heads are spread over blocks too, down to one step a warp. A backward that sums scale
-// gradients keeps to a fixed number of blocks, which walk the tokens.
+// A block's four warps hold 4 tokens, or fewer with several warps a token where that leaves less than six blocks an SM:
+// more tokens a block share the table's cost, more blocks fill the SMs. Forward, us with three / six / twelve blocks:
+//   48 heads x 128   1900 tokens 18.8 / 12.0 / 13.2   3300 19.4 / 17.7 / 19.4   4608 20.6 / 20.6 / 22.3   6000 32.8 / 32.8 / 30.9
+//   16 heads x 64    1900 tokens 7.9 / 6.2 / 8.9      3300 8.3 / 8.7 / 13.3     4608 8.4 / 8.4 / 10.5     6000 11.0 / 11.0 / 12.9
+// A lone token's heads are spread over blocks too, down to one step a warp. A backward that sums scale gradients keeps to
+// a fixed number of blocks, which walk the tokens.
 static dim3 plan(RopeArgs* a, int rows, int sms) {
   const long long tokens = (long long)a->B * a->L;
   const int steps = (a->heads[0] + rows - 1) / rows + (a->heads[1] + rows - 1) / rows;
